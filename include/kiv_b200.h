@@ -84,6 +84,10 @@ typedef int32_t kiv_status;
 #define KIV_ERRBIT_CAND_CAPACITY 4    /* candidates larger than the workspace */
 #define KIV_ERRBIT_WAIT_TIMEOUT 8     /* a bounded wait on a bulk copy gave up */
 #define KIV_ERRBIT_STAGE_CAPACITY 16  /* more host pages in the union than staging pages */
+/* the paged and rotation calls set these in their `errors` word */
+#define KIV_ERRBIT_BLOCK_TABLE 32     /* a page number that a live token needs is outside [0, num_pages) */
+#define KIV_ERRBIT_SEQ_LEN 64         /* a length below its new tokens' count, or above table_width * page_size */
+#define KIV_ERRBIT_POSITION 128       /* a position (or pair axis) outside the cos / sin table */
 
 typedef struct kiv_store {
   int32_t batch;
@@ -390,6 +394,117 @@ KIV_API kiv_status kiv_attend_peers(const kiv_store *st, const kiv_query *q, con
  * this rank's [B*Hq*Q, D + 4] from kiv_attend. */
 KIV_API kiv_status kiv_attend_exchange_merge(const kiv_store *st, const kiv_query *q, const float *partial,
                                              const kiv_exchange *x, void *out, void *stream);
+
+/*
+ * Paged cache of a batch of sequences of unequal lengths, and the turn (norm
+ * and rotation) of query and key rows in front of it.  No counterpart in the
+ * reference: its caches are dense and hold one batch of equal lengths; these
+ * calls serve next to them where an engine keeps its hot tier in pages.
+ *
+ * k, v         [num_pages, Hkv, page_size, D], any strides, D contiguous, rows
+ *              16-byte aligned (an engine's [blocks, page_size, Hkv, D] tensor
+ *              is the same thing with other strides)
+ * block_table  [batch, table_width] page numbers: token j of sequence b lies in
+ *              page block_table[b][j / page_size] at row j % page_size
+ * seq_lens     [batch] tokens of each sequence, the new ones included
+ * q_starts     [batch + 1] row of each sequence's first new token among the
+ *              num_tokens packed rows; sequence b has n_b = q_starts[b+1] -
+ *              q_starts[b] new tokens, its last n_b.  Rows from q_starts[batch]
+ *              on (a padded batch) are neither read nor written.
+ * The three arrays are device memory and are read by the kernels, so a
+ * captured call serves changing lengths and pages.  Page numbers outside
+ * [0, num_pages) are never followed: see the calls.
+ */
+typedef struct kiv_paged {
+  int32_t batch, num_kv_heads, head_dim, page_size, dtype;
+  int32_t max_query_len;    /* largest n_b if the host knows it, else 0: picks kernels, never results */
+  int64_t num_pages;
+  void *k, *v;
+  int64_t k_stride_p, k_stride_h, k_stride_t;   /* elements */
+  int64_t v_stride_p, v_stride_h, v_stride_t;
+  const int32_t *block_table;
+  int64_t table_stride, table_width;
+  const int32_t *seq_lens, *q_starts;
+  int64_t num_tokens;
+  int64_t *errors;          /* device word that collects KIV_ERRBIT_* (never cleared here), or NULL */
+} kiv_paged;
+
+/* Norm and rotation of rows: y = x * rsqrt(mean(x^2) + eps) * (weight_offset +
+ * weight) (norm != 0; no weight: * 1), then each pair (a, b) of the first
+ * rot_dim elements turns to (a cos - b sin, b cos + a sin).  Pair j is elements
+ * (j, j + rot_dim/2), or (2j, 2j+1) when interleaved.  cos / sin [cs_rows,
+ * rot_dim/2]; the row for pair j is positions[axis of j], the axis being
+ * pair_axes[j] (0 without pair_axes).  Computed in fp32, rounded once. */
+typedef struct kiv_turn {
+  const void *cos, *sin;    /* NULL: no rotation */
+  int64_t cs_stride, cs_rows;
+  int32_t cs_dtype;         /* KIV_DTYPE_F32 or the rows' dtype */
+  int32_t rot_dim;          /* even, <= head_dim */
+  const void *positions;    /* [axes, batch, tokens] (append: [axes, num_tokens]) or NULL */
+  int64_t pos_stride_a, pos_stride_b, pos_stride_t;
+  int32_t pos_is_i64;       /* 1: int64 positions, 0: int32 */
+  int32_t axes;             /* >= 1 */
+  const int32_t *pair_axes; /* [rot_dim / 2] or NULL */
+  int32_t interleaved;
+  int32_t norm;
+  float eps, weight_offset;
+  const void *q_weight, *k_weight;   /* [D] or NULL */
+  int32_t weight_dtype;     /* KIV_DTYPE_F32 or the rows' dtype */
+  int32_t reserved;
+} kiv_turn;
+
+/* Rows [batch, heads, tokens, D], D contiguous, 16-byte aligned; strides in elements. */
+typedef struct kiv_rows {
+  void *p;
+  int64_t stride_b, stride_h, stride_t;
+  int32_t heads;
+  int32_t reserved;
+} kiv_rows;
+
+/*
+ * Turn the query rows q and (k not NULL) key rows k into q_out and k_out, which
+ * may be the inputs themselves.  Without positions the row of the cos / sin
+ * table is b * tokens + t (tables already gathered per token).  A row whose
+ * position lies outside the table is written as NaN.
+ */
+KIV_API kiv_status kiv_qk_norm_rope(int32_t dtype, int32_t batch, int32_t tokens, int32_t head_dim,
+                                    const kiv_rows *q, const kiv_rows *k, const kiv_rows *q_out,
+                                    const kiv_rows *k_out, const kiv_turn *turn, int64_t *errors, void *stream);
+
+/*
+ * Write the new tokens' rows k, v ([num_tokens, Hkv, D]) to their places in the
+ * pages, the keys turned on the way (turn NULL: copied).  Without positions a
+ * key turns by its place in the sequence.  A token whose place has no page, or
+ * whose position lies outside the table, is not written.
+ * Two tokens with the same place (a page shared by two table rows) race.
+ */
+KIV_API kiv_status kiv_paged_append(const kiv_paged *pc, const void *k, int64_t k_stride_t, int64_t k_stride_h,
+                                    const void *v, int64_t v_stride_t, int64_t v_stride_h, const kiv_turn *turn,
+                                    void *stream);
+
+typedef struct kiv_paged_query {
+  const void *q;            /* [num_tokens, Hq, D], cache dtype, D contiguous */
+  int64_t stride_t, stride_h;
+  void *out;                /* [num_tokens, Hq, D] */
+  int64_t out_stride_t, out_stride_h;
+  float *lse;               /* [num_tokens, Hq] contiguous, or NULL */
+  int32_t num_query_heads;
+  int32_t causal;           /* 1: new token i of sequence b sees keys j <= seq_lens[b] - n_b + i; 0: all */
+  int32_t window;           /* > 0 (causal only): it sees only the last `window` of those */
+  float scaling, softcap;   /* score = softcap * tanh(scaling * <q, k> / softcap), or without softcap (0) */
+} kiv_paged_query;
+
+/*
+ * Attention of every sequence's new tokens over its keys in the pages.  lse is
+ * the natural logarithm of the sum of exp(score).  A row that sees no key gets
+ * out 0 and lse -inf.  Keys whose page number is outside [0, num_pages) read as
+ * rows of zeros.  Rows of the pages past a sequence's length, and of pages no
+ * row of a tile sees, never reach a result, whatever they hold.
+ * Results do not depend on the order in which the GPU runs the blocks.
+ */
+KIV_API size_t kiv_paged_workspace_bytes(const kiv_paged *pc, const kiv_paged_query *q);
+KIV_API kiv_status kiv_paged_attend(const kiv_paged *pc, const kiv_paged_query *q, void *ws, size_t ws_bytes,
+                                    void *stream);
 
 /* Copy the store's device state words to host memory (synchronizes the stream). */
 KIV_API kiv_status kiv_read_state(const kiv_store *st, int64_t *host_words, void *stream);

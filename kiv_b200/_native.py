@@ -72,6 +72,40 @@ class PeerRows(ctypes.Structure):
     _fields_ = [("cold_k", c_vp * MAX_PEERS), ("cold_v", c_vp * MAX_PEERS)]
 
 
+class PagedDesc(ctypes.Structure):
+    """kiv_paged: a paged cache and the new tokens' rows of a batch."""
+    _fields_ = [("batch", c_i32), ("num_kv_heads", c_i32), ("head_dim", c_i32), ("page_size", c_i32), ("dtype", c_i32),
+                ("max_query_len", c_i32), ("num_pages", c_i64), ("k", c_vp), ("v", c_vp),
+                ("k_stride_p", c_i64), ("k_stride_h", c_i64), ("k_stride_t", c_i64),
+                ("v_stride_p", c_i64), ("v_stride_h", c_i64), ("v_stride_t", c_i64),
+                ("block_table", c_vp), ("table_stride", c_i64), ("table_width", c_i64),
+                ("seq_lens", c_vp), ("q_starts", c_vp), ("num_tokens", c_i64), ("errors", c_vp)]
+
+
+class TurnDesc(ctypes.Structure):
+    """kiv_turn: norm and rotation of rows."""
+    _fields_ = [("cos", c_vp), ("sin", c_vp), ("cs_stride", c_i64), ("cs_rows", c_i64), ("cs_dtype", c_i32),
+                ("rot_dim", c_i32), ("positions", c_vp), ("pos_stride_a", c_i64), ("pos_stride_b", c_i64),
+                ("pos_stride_t", c_i64), ("pos_is_i64", c_i32), ("axes", c_i32), ("pair_axes", c_vp),
+                ("interleaved", c_i32), ("norm", c_i32), ("eps", c_f32), ("weight_offset", c_f32),
+                ("q_weight", c_vp), ("k_weight", c_vp), ("weight_dtype", c_i32), ("reserved", c_i32)]
+
+
+class RowsDesc(ctypes.Structure):
+    """kiv_rows: [batch, heads, tokens, D] rows."""
+    _fields_ = [("p", c_vp), ("stride_b", c_i64), ("stride_h", c_i64), ("stride_t", c_i64), ("heads", c_i32),
+                ("reserved", c_i32)]
+
+
+class PagedQueryDesc(ctypes.Structure):
+    """kiv_paged_query: the queries of kiv_paged_attend and where its results go."""
+    _fields_ = [("q", c_vp), ("stride_t", c_i64), ("stride_h", c_i64), ("out", c_vp), ("out_stride_t", c_i64),
+                ("out_stride_h", c_i64), ("lse", c_vp), ("num_query_heads", c_i32), ("causal", c_i32),
+                ("window", c_i32), ("scaling", c_f32), ("softcap", c_f32)]
+
+
+ERRBIT_BLOCK_TABLE, ERRBIT_SEQ_LEN, ERRBIT_POSITION = 32, 64, 128
+
 P = ctypes.POINTER
 # name -> (restype, argtypes)
 SIGNATURES = {
@@ -114,6 +148,11 @@ SIGNATURES = {
                                  c_vp, c_vp]),
     "kiv_fine_exchange_select": (c_i32, [P(StoreDesc), P(QueryDesc), c_vp, c_sz, P(ExchangeDesc), c_vp, c_vp,
                                          c_vp]),
+    "kiv_qk_norm_rope": (c_i32, [c_i32, c_i32, c_i32, c_i32, P(RowsDesc), P(RowsDesc), P(RowsDesc), P(RowsDesc),
+                                 P(TurnDesc), c_vp, c_vp]),
+    "kiv_paged_append": (c_i32, [P(PagedDesc), c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, P(TurnDesc), c_vp]),
+    "kiv_paged_workspace_bytes": (c_sz, [P(PagedDesc), P(PagedQueryDesc)]),
+    "kiv_paged_attend": (c_i32, [P(PagedDesc), P(PagedQueryDesc), c_vp, c_sz, c_vp]),
 }
 
 _lib = None

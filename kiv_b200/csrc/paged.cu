@@ -1,0 +1,453 @@
+// Attention of new tokens over a paged cache (kiv_paged_attend): checks,
+// choice of kernel, the CUDA-core kernel, and the join of split items.
+//
+//   out = softmax(score(q k^T)) v over the keys a token sees, one pass over
+//   the keys with the running maximum and sum of each row in fp32.
+#include <algorithm>
+
+#include "internal.h"
+#include "paged.cuh"
+
+namespace kiv {
+
+kiv_status check_paged(const kiv_paged *pc) {
+  if (!pc) { set_error("paged cache is NULL"); return KIV_ERR_ARG; }
+  if (pc->dtype < 0 || pc->dtype > 2) { set_error("unknown dtype %d", pc->dtype); return KIV_ERR_UNSUPPORTED; }
+  const int eb = elem_bytes(pc->dtype);
+  if (pc->batch < 0 || pc->num_kv_heads < 1 || pc->head_dim < 1 || pc->page_size < 1 || pc->num_pages < 0 ||
+      pc->table_width < 0 || pc->table_stride < 0 || pc->num_tokens < 0 || pc->max_query_len < 0) {
+    set_error("bad paged cache sizes");
+    return KIV_ERR_ARG;
+  }
+  if ((pc->head_dim * eb) % 16 != 0) {
+    set_error("head_dim %d: rows must be a multiple of 16 bytes", pc->head_dim);
+    return KIV_ERR_UNSUPPORTED;
+  }
+  if (pc->num_tokens > 0x7fffffff || pc->num_pages > 0x7fffffff || pc->table_width > 0x7fffffff / pc->page_size ||
+      pc->batch > (1 << 20)) {
+    set_error("paged cache too large: tokens, pages and table_width * page_size stay below 2^31, batch at most 2^20");
+    return KIV_ERR_UNSUPPORTED;
+  }
+  if (pc->num_tokens > 0 && pc->batch > 0 &&
+      (!pc->seq_lens || !pc->q_starts || (pc->table_width > 0 && !pc->block_table))) {
+    set_error("block_table, seq_lens or q_starts missing");
+    return KIV_ERR_ARG;
+  }
+  const int64_t strides[6] = {pc->k_stride_p, pc->k_stride_h, pc->k_stride_t, pc->v_stride_p, pc->v_stride_h, pc->v_stride_t};
+  for (int64_t s : strides)
+    if (s < 0 || (s * eb) % 16) { set_error("page strides must be multiples of 16 bytes"); return KIV_ERR_ARG; }
+  if (pc->num_pages > 0 && (!pc->k || !pc->v || (reinterpret_cast<uintptr_t>(pc->k) & 15) || (reinterpret_cast<uintptr_t>(pc->v) & 15))) {
+    set_error("pages missing or not 16-byte aligned");
+    return KIV_ERR_ARG;
+  }
+  return KIV_OK;
+}
+
+static kiv_status check_paged_query(const kiv_paged *pc, const kiv_paged_query *q) {
+  if (!q) { set_error("paged query is NULL"); return KIV_ERR_ARG; }
+  const int eb = elem_bytes(pc->dtype);
+  if (q->num_query_heads < 1 || q->num_query_heads % pc->num_kv_heads != 0) {
+    set_error("query heads %d are not a multiple of key heads %d", q->num_query_heads, pc->num_kv_heads);
+    return KIV_ERR_ARG;
+  }
+  if (pc->head_dim > 256) { set_error("paged attention: head_dim %d above 256", pc->head_dim); return KIV_ERR_UNSUPPORTED; }
+  if (q->window < 0 || (q->window > 0 && !q->causal)) { set_error("window must not be negative, and needs causal"); return KIV_ERR_ARG; }
+  if (!(q->softcap >= 0.f)) { set_error("softcap must not be negative"); return KIV_ERR_ARG; }
+  if (pc->num_tokens > 0 &&
+      (!q->q || !q->out || (reinterpret_cast<uintptr_t>(q->q) & 15) || (reinterpret_cast<uintptr_t>(q->out) & 15) ||
+       (q->stride_t * eb) % 16 || (q->stride_h * eb) % 16 || (q->out_stride_t * eb) % 16 || (q->out_stride_h * eb) % 16)) {
+    set_error("query or output rows missing or not 16-byte aligned");
+    return KIV_ERR_ARG;
+  }
+  return KIV_OK;
+}
+
+// ---------------------------------------------------------------------------
+// CUDA-core kernel: fp32 rows (tensor cores would round them) and head
+// dimensions outside the tensor-core kernels' set.  R rows x 64 keys per
+// step; 16 threads share a row, each with 4 keys of the scores and a sixteenth
+// of the output row.  Bound by the shared-memory reads that feed the FMAs
+// (a 4 x 4 register tile: 8 FMAs per 16 bytes read).
+// ---------------------------------------------------------------------------
+constexpr int CC_KEYS = 64;
+constexpr int CC_THREADS = 256;
+
+template <int R>
+static size_t cc_smem(int D) {
+  return sizeof(float) * ((size_t)(R + 2 * CC_KEYS) * (D + 4) + (size_t)R * (CC_KEYS + 4));
+}
+
+template <typename T, int R, int DM>
+__global__ void __launch_bounds__(CC_THREADS) paged_cc_kernel(const __grid_constant__ PagedPlan p) {
+  constexpr int V = Elem<T>::V;
+  constexpr int RPT = R / 16;          // rows per thread
+  constexpr int DC = (DM + 63) / 64;   // 4-element slices of an output row per thread
+  extern __shared__ float4 cc_dyn[];
+  __shared__ int64_t sm[40];
+  __shared__ int64_t s_ko[CC_KEYS], s_vo[CC_KEYS];
+  const int D = p.pc.head_dim, nv = D / V, ld = D + 4;
+  float *sq = reinterpret_cast<float *>(cc_dyn);
+  float *sk = sq + R * ld, *sv = sk + CC_KEYS * ld, *sp = sv + CC_KEYS * ld;
+  const int tr = threadIdx.x / 16, tc = threadIdx.x % 16;
+  griddep_wait();
+  PagedSpot at = paged_locate<CC_THREADS>(p, blockIdx.x, gridDim.x, sm);
+  const int64_t end = (int64_t)(blockIdx.x + 1) * at.total / gridDim.x;
+  if (threadIdx.x == 0) p.cut[blockIdx.x].b = -1;
+  while (at.it.s.b >= 0 && at.unit < end) {
+    const PagedSegment g = paged_segment(p, at, end);
+    const int kvh = at.hp / p.hs;
+    int lo, hi;
+    paged_range(p, at.it, at.rt, lo, hi);
+    if (threadIdx.x == 0) {
+      if (!g.head) paged_check_lens(p.pc, at.it.s);
+      if (g.tail) paged_record(p, blockIdx.x, at, g);
+    }
+    hi = min(hi, at.it.s.len);
+    __syncthreads();
+    for (int x = threadIdx.x; x < R * nv; x += CC_THREADS) {
+      const int r = x / nv, vi = x - r * nv;
+      float f[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) f[e] = 0.f;
+      int i, head;
+      if (paged_row(p, at.it, at.hp, at.rt, r, i, head))
+        Elem<T>::unpack(ld16(static_cast<const T *>(p.q.q) + (at.it.s.q0 + i) * p.q.stride_t + head * p.q.stride_h + vi * V), f);
+#pragma unroll
+      for (int e = 0; e < V; ++e) sq[r * ld + vi * V + e] = f[e];
+    }
+    int place[RPT];                    // of each row's token; -1: no such row
+    bool have[RPT];
+    float m[RPT], l[RPT];
+    float4 o[RPT][DC];
+#pragma unroll
+    for (int a = 0; a < RPT; ++a) {
+      int i, head;
+      have[a] = paged_row(p, at.it, at.hp, at.rt, tr * RPT + a, i, head);
+      place[a] = p.q.causal ? at.it.base + i : 0x7fffffff;
+      m[a] = -INFINITY;
+      l[a] = 0.f;
+#pragma unroll
+      for (int c = 0; c < DC; ++c) o[a][c] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    for (int t = g.t0; t < g.t1; ++t) {
+      const int64_t j0 = ((int64_t)lo / CC_KEYS + t) * CC_KEYS;
+      __syncthreads();                 // the previous step's readers are done
+      if (threadIdx.x < CC_KEYS) {
+        const int64_t j = j0 + threadIdx.x;
+        int64_t ko = -1, vo = -1;
+        if (j >= lo && j < hi) {
+          paged_key(p.pc, at.it.s.b, j, kvh, ko, vo);
+          if (ko < 0) paged_error(p.pc.errors, KIV_ERRBIT_BLOCK_TABLE);
+        }
+        s_ko[threadIdx.x] = ko;
+        s_vo[threadIdx.x] = vo;
+      }
+      __syncthreads();
+      for (int x = threadIdx.x; x < 2 * CC_KEYS * nv; x += CC_THREADS) {
+        const bool isv = x >= CC_KEYS * nv;
+        const int y = isv ? x - CC_KEYS * nv : x;
+        const int r = y / nv, vi = y - r * nv;
+        const int64_t off = isv ? s_vo[r] : s_ko[r];
+        float f[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) f[e] = 0.f;
+        if (off >= 0) Elem<T>::unpack(ld16(static_cast<const T *>(isv ? p.pc.v : p.pc.k) + off + vi * V), f);
+        float *d = (isv ? sv : sk) + r * ld + vi * V;
+#pragma unroll
+        for (int e = 0; e < V; ++e) d[e] = f[e];
+      }
+      __syncthreads();
+      float s[RPT][4];
+#pragma unroll
+      for (int a = 0; a < RPT; ++a)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) s[a][c] = 0.f;
+      for (int d = 0; d < D; d += 4) {
+        float4 kk[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) kk[c] = *reinterpret_cast<const float4 *>(sk + (tc + 16 * c) * ld + d);
+#pragma unroll
+        for (int a = 0; a < RPT; ++a) {
+          const float4 qq = *reinterpret_cast<const float4 *>(sq + (tr * RPT + a) * ld + d);
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            s[a][c] = fmaf(qq.x, kk[c].x, fmaf(qq.y, kk[c].y, fmaf(qq.z, kk[c].z, fmaf(qq.w, kk[c].w, s[a][c]))));
+        }
+      }
+#pragma unroll
+      for (int a = 0; a < RPT; ++a) {
+        float mx = m[a];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int64_t j = j0 + tc + 16 * c;
+          float x = s[a][c] * p.q.scaling;
+          if (p.q.softcap > 0.f) x = p.q.softcap * tanhf(x / p.q.softcap);
+          const bool seen = j < hi && j <= place[a] && (p.q.window == 0 || j > (int64_t)place[a] - p.q.window);
+          s[a][c] = seen ? x : -INFINITY;
+          mx = fmaxf(mx, s[a][c]);
+        }
+#pragma unroll
+        for (int w = 8; w > 0; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(KIV_FULL_MASK, mx, w));
+        const float ms = mx == -INFINITY ? 0.f : mx;     // a row that has seen nothing yet: exp(-inf) = 0
+        const float keep = exp2f((m[a] - ms) * 1.44269504f);
+        float sum = 0.f;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const float e = exp2f((s[a][c] - ms) * 1.44269504f);
+          sp[(tr * RPT + a) * (CC_KEYS + 4) + tc + 16 * c] = e;
+          sum += e;
+        }
+#pragma unroll
+        for (int w = 8; w > 0; w >>= 1) sum += __shfl_xor_sync(KIV_FULL_MASK, sum, w);
+        l[a] = l[a] * keep + sum;
+        m[a] = mx;
+#pragma unroll
+        for (int c = 0; c < DC; ++c) {
+          o[a][c].x *= keep;
+          o[a][c].y *= keep;
+          o[a][c].z *= keep;
+          o[a][c].w *= keep;
+        }
+      }
+      __syncwarp();                    // a row's 16 threads are in one warp
+#pragma unroll 1
+      for (int j = 0; j < CC_KEYS; j += 4) {
+        float4 pp[RPT];
+#pragma unroll
+        for (int a = 0; a < RPT; ++a) pp[a] = *reinterpret_cast<const float4 *>(sp + (tr * RPT + a) * (CC_KEYS + 4) + j);
+#pragma unroll
+        for (int jj = 0; jj < 4; ++jj) {
+#pragma unroll
+          for (int c = 0; c < DC; ++c) {
+            const int d = 4 * tc + 64 * c;
+            if (d < D) {
+              const float4 vv = *reinterpret_cast<const float4 *>(sv + (j + jj) * ld + d);
+#pragma unroll
+              for (int a = 0; a < RPT; ++a) {
+                const float e = jj == 0 ? pp[a].x : jj == 1 ? pp[a].y : jj == 2 ? pp[a].z : pp[a].w;
+                o[a][c].x = fmaf(e, vv.x, o[a][c].x);
+                o[a][c].y = fmaf(e, vv.y, o[a][c].y);
+                o[a][c].z = fmaf(e, vv.z, o[a][c].z);
+                o[a][c].w = fmaf(e, vv.w, o[a][c].w);
+              }
+            }
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int a = 0; a < RPT; ++a) {
+      if (!have[a]) continue;
+      const int r = tr * RPT + a;
+      int i, head;
+      paged_row(p, at.it, at.hp, at.rt, r, i, head);
+      if (!g.head && !g.tail) {
+        const float inv = l[a] > 0.f ? 1.f / l[a] : 0.f;
+        T *dst = paged_out<T>(p, at.it, i, head);
+#pragma unroll
+        for (int c = 0; c < DC; ++c) {
+          const int d = 4 * tc + 64 * c;
+          if (d < D) {
+            dst[d] = Elem<T>::from_f(o[a][c].x * inv);
+            dst[d + 1] = Elem<T>::from_f(o[a][c].y * inv);
+            dst[d + 2] = Elem<T>::from_f(o[a][c].z * inv);
+            dst[d + 3] = Elem<T>::from_f(o[a][c].w * inv);
+          }
+        }
+        if (tc == 0) paged_lse(p, at.it, i, head, m[a], l[a]);
+      } else {
+        float *dst = paged_part(p, 2 * (int64_t)blockIdx.x + (g.head ? 0 : 1), r);
+#pragma unroll
+        for (int c = 0; c < DC; ++c)
+          if (4 * tc + 64 * c < D) *reinterpret_cast<float4 *>(dst + 4 * tc + 64 * c) = o[a][c];
+        if (tc == 0) {
+          dst[D] = m[a];
+          dst[D + 1] = l[a];
+        }
+      }
+    }
+    at.unit += g.t1 - g.t0;
+    if (g.tail) break;
+    paged_next(p, at);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Join of the items that blocks share.  Block (c, y) takes the item that block
+// c of the attention kernel began and did not finish; a warp takes a row's
+// slice of 128 columns: the parts' maxima first, then their scaled sum, in
+// block order.
+// ---------------------------------------------------------------------------
+constexpr int CB_WARPS = 8;
+
+template <typename T>
+__global__ void __launch_bounds__(CB_WARPS * 32) paged_combine_kernel(const __grid_constant__ PagedPlan p, int blocks) {
+  griddep_wait();
+  const PagedCut cut = p.cut[blockIdx.x];
+  if (cut.b < 0) return;
+  const int D = p.pc.head_dim, lane = threadIdx.x & 31;
+  const int slices = (D + 127) / 128;
+  const PagedItems it = paged_items(p, cut.b);
+  const int warp = (blockIdx.y * CB_WARPS + (threadIdx.x >> 5)), nwarps = gridDim.y * CB_WARPS;
+  // parts: slot 2c + 1, then slot 2c' of each later block whose stretch begins inside the item
+  const int c0 = blockIdx.x;
+  int last = c0;
+  {
+    // block c' takes part while its stretch begins before the item's end: c' N / G < end
+    int a = c0, z = blocks;            // a takes part, z does not
+    while (z - a > 1) {
+      const int mid = (a + z) / 2;
+      if ((int64_t)mid * cut.total / blocks < cut.end) a = mid; else z = mid;
+    }
+    last = a;
+  }
+  for (int x = warp; x < p.tpt * p.grp * slices; x += nwarps) {
+    const int r = x / slices, col = (x % slices) * 128 + 4 * lane;
+    int i, head;
+    if (!paged_row(p, it, cut.hp, cut.rt, r, i, head)) continue;
+    float mx = -INFINITY;
+    for (int c = c0 + lane; c <= last; c += 32) {
+      // a block with an empty stretch (fewer tiles than blocks) left nothing
+      if ((int64_t)c * cut.total / blocks == (int64_t)(c + 1) * cut.total / blocks) continue;
+      mx = fmaxf(mx, paged_part(p, 2 * (int64_t)c + (c == c0), r)[D]);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(KIV_FULL_MASK, mx, o));
+    const float ms = mx == -INFINITY ? 0.f : mx;
+    float l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int c = c0; c <= last; ++c) {
+      if ((int64_t)c * cut.total / blocks == (int64_t)(c + 1) * cut.total / blocks) continue;
+      const float *src = paged_part(p, 2 * (int64_t)c + (c == c0), r);
+      const float w = exp2f((src[D] - ms) * 1.44269504f);
+      l = fmaf(src[D + 1], w, l);
+      if (col < D) {
+        const float4 v = *reinterpret_cast<const float4 *>(src + col);
+        acc.x = fmaf(v.x, w, acc.x);
+        acc.y = fmaf(v.y, w, acc.y);
+        acc.z = fmaf(v.z, w, acc.z);
+        acc.w = fmaf(v.w, w, acc.w);
+      }
+    }
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    if (col < D) {
+      T *dst = paged_out<T>(p, it, i, head) + col;
+      dst[0] = Elem<T>::from_f(acc.x * inv);
+      dst[1] = Elem<T>::from_f(acc.y * inv);
+      dst[2] = Elem<T>::from_f(acc.z * inv);
+      dst[3] = Elem<T>::from_f(acc.w * inv);
+    }
+    if (lane == 0 && x % slices == 0) paged_lse(p, it, i, head, mx, l);
+  }
+}
+
+kiv_status launch_paged_combine(const PagedPlan &p, int blocks, cudaStream_t s) {
+  if (blocks < 2) return KIV_OK;
+  const int slices = (int)ceil_div(p.pc.head_dim, 128);
+  const int y = (int)std::min<int64_t>(ceil_div((int64_t)p.tpt * p.grp * slices, CB_WARPS), 8);
+  const dim3 grid((unsigned)blocks, (unsigned)y), block(CB_WARPS * 32);
+  cudaError_t e;
+  if (p.pc.dtype == KIV_DTYPE_F32) e = launch_pdl(paged_combine_kernel<float>, grid, block, 0, s, 1, p, blocks);
+  else if (p.pc.dtype == KIV_DTYPE_BF16) e = launch_pdl(paged_combine_kernel<__nv_bfloat16>, grid, block, 0, s, 1, p, blocks);
+  else e = launch_pdl(paged_combine_kernel<__half>, grid, block, 0, s, 1, p, blocks);
+  return cuda_status(e, "paged_combine");
+}
+
+// ------------------------------------------------------------------ host
+// Tiling of one kernel's items: `rows` rows per tile, `kt` keys per tile.
+static PagedPlan make_plan(const kiv_paged *pc, const kiv_paged_query *q, int rows, int kt) {
+  PagedPlan p = {};
+  p.pc = *pc;
+  p.q = *q;
+  const int per = q->num_query_heads / pc->num_kv_heads;
+  p.hs = (int)ceil_div(per, rows);
+  p.grp = (int)ceil_div(per, p.hs);
+  p.tpt = rows / p.grp;
+  p.kt = kt;
+  p.rows = rows;
+  p.min_rows = 0;
+  p.max_rows = 0x7fffffff;
+  return p;
+}
+
+struct PagedCall {
+  PagedPlan p;
+  int blocks;
+  size_t bytes;        // of its workspace
+  size_t cut_offset;
+};
+
+static void size_call(PagedCall &c) {
+  c.cut_offset = (size_t)align_up((int64_t)2 * c.blocks * c.p.rows * partial_stride(c.p.pc.head_dim) * 4, 256);
+  c.bytes = c.cut_offset + (size_t)align_up((int64_t)c.blocks * sizeof(PagedCut), 256);
+}
+
+// rows a sequence of the largest (or, unknown, the average) length brings per key head
+static int64_t likely_rows(const kiv_paged *pc, const kiv_paged_query *q) {
+  const int64_t per = q->num_query_heads / pc->num_kv_heads;
+  const int64_t n = pc->max_query_len > 0 ? pc->max_query_len : ceil_div(pc->num_tokens, std::max(1, pc->batch));
+  return per * n;
+}
+
+static PagedCall plan_cc(const kiv_paged *pc, const kiv_paged_query *q) {
+  PagedCall c;
+  const int rows = likely_rows(pc, q) <= 16 ? 16 : 64;
+  c.p = make_plan(pc, q, rows, CC_KEYS);
+  const size_t smem = rows == 16 ? cc_smem<16>(pc->head_dim) : cc_smem<64>(pc->head_dim);
+  c.blocks = sm_count() * (int)std::max<size_t>(1, std::min<size_t>(4, (220 * 1024) / (smem + 2048)));
+  size_call(c);
+  return c;
+}
+
+template <typename T, int R, int DM>
+static cudaError_t launch_cc(const PagedCall &c, cudaStream_t s) {
+  const size_t smem = cc_smem<R>(c.p.pc.head_dim);
+  cudaFuncSetAttribute(paged_cc_kernel<T, R, DM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  return launch_pdl(paged_cc_kernel<T, R, DM>, dim3((unsigned)c.blocks), dim3(CC_THREADS), smem, s, 1, c.p);
+}
+template <typename T, int R>
+static cudaError_t launch_cc_d(const PagedCall &c, cudaStream_t s) {
+  const int D = c.p.pc.head_dim;
+  return D <= 64 ? launch_cc<T, R, 64>(c, s) : D <= 128 ? launch_cc<T, R, 128>(c, s) : launch_cc<T, R, 256>(c, s);
+}
+template <typename T>
+static cudaError_t launch_cc_r(const PagedCall &c, cudaStream_t s) {
+  return c.p.rows == 16 ? launch_cc_d<T, 16>(c, s) : launch_cc_d<T, 64>(c, s);
+}
+
+static kiv_status run_cc(PagedCall c, char *ws, cudaStream_t s) {
+  c.p.part = reinterpret_cast<float *>(ws);
+  c.p.cut = reinterpret_cast<PagedCut *>(ws + c.cut_offset);
+  cudaError_t e;
+  if (c.p.pc.dtype == KIV_DTYPE_F32) e = launch_cc_r<float>(c, s);
+  else if (c.p.pc.dtype == KIV_DTYPE_BF16) e = launch_cc_r<__nv_bfloat16>(c, s);
+  else e = launch_cc_r<__half>(c, s);
+  KIV_CHECK(cuda_status(e, "paged_attend"));
+  return launch_paged_combine(c.p, c.blocks, s);
+}
+
+}  // namespace kiv
+
+using namespace kiv;
+
+extern "C" {
+
+size_t kiv_paged_workspace_bytes(const kiv_paged *pc, const kiv_paged_query *q) {
+  if (check_paged(pc) != KIV_OK || !q || q->num_query_heads < 1 || q->num_query_heads % pc->num_kv_heads || pc->head_dim > 256) return 0;
+  return plan_cc(pc, q).bytes;
+}
+
+kiv_status kiv_paged_attend(const kiv_paged *pc, const kiv_paged_query *q, void *ws, size_t ws_bytes, void *stream) {
+  KIV_CHECK(check_paged(pc));
+  KIV_CHECK(check_paged_query(pc, q));
+  if (pc->num_tokens == 0 || pc->batch == 0) return KIV_OK;
+  const PagedCall c = plan_cc(pc, q);
+  if (!ws || ws_bytes < c.bytes || (reinterpret_cast<uintptr_t>(ws) & 255)) {
+    set_error("workspace too small or misaligned (%zu < %zu)", ws_bytes, c.bytes);
+    return KIV_ERR_CAPACITY;
+  }
+  return run_cc(c, static_cast<char *>(ws), (cudaStream_t)stream);
+}
+
+}  // extern "C"

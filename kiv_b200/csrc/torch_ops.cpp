@@ -17,9 +17,11 @@
 // The operators that write return nothing and declare what they mutate in
 // their schema.  Failures raise RuntimeError with the library's message.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/ops/empty.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <cstdint>
 #include <vector>
 
@@ -338,6 +340,218 @@ void attend_exchange_merge(at::TensorList store, at::IntArrayRef geom, const Ten
         "attend_exchange_merge");
 }
 
+// ------------------------------------------------- rotation and paged cache
+void check_same(const Tensor &a, const Tensor &t, const char *what) {
+  TORCH_CHECK(t.device() == a.device(), "kiv: ", what, " is on ", t.device(), ", the rows are on ", a.device());
+}
+
+int64_t *error_word(const Tensor &a, const c10::optional<Tensor> &errors) {
+  if (!errors.has_value() || !errors->defined()) return nullptr;
+  check_same(a, *errors, "errors");
+  TORCH_CHECK(errors->scalar_type() == at::kLong && errors->numel() >= 1, "kiv: errors must be an int64 tensor");
+  return errors->data_ptr<int64_t>();
+}
+
+// stride of a dimension; one of size 1 is never stepped, whatever its stride says
+int64_t step(const Tensor &t, int d) { return t.size(d) == 1 ? 0 : t.stride(d); }
+
+const Tensor *given(const c10::optional<Tensor> &t) { return t.has_value() && t->defined() ? &*t : nullptr; }
+
+// lead: dimensions of positions behind the axes ([batch, tokens] or [num_tokens])
+kiv_turn make_turn(const Tensor &rows, int64_t head_dim, const c10::optional<Tensor> &cos, const c10::optional<Tensor> &sin,
+                   const c10::optional<Tensor> &positions, const c10::optional<Tensor> &pair_axes, bool interleaved,
+                   c10::optional<double> eps, const c10::optional<Tensor> &q_weight, const c10::optional<Tensor> &k_weight,
+                   double weight_offset, at::IntArrayRef lead, bool rows_given) {
+  kiv_turn t = {};
+  t.axes = 1;
+  TORCH_CHECK((given(cos) != nullptr) == (given(sin) != nullptr), "kiv: cos and sin come together");
+  if (const Tensor *c = given(cos)) {
+    const Tensor &s = *given(sin);
+    check_same(rows, *c, "cos");
+    check_same(rows, s, "sin");
+    TORCH_CHECK(c->dim() == 2 && s.sizes() == c->sizes() && s.strides() == c->strides() && c->stride(1) == 1,
+                "kiv: cos and sin must be [rows, rot_dim / 2] alike, with a contiguous last dim");
+    TORCH_CHECK(s.scalar_type() == c->scalar_type(), "kiv: cos and sin must have one dtype");
+    t.cos = c->data_ptr();
+    t.sin = s.data_ptr();
+    t.cs_stride = c->stride(0);
+    t.cs_rows = c->size(0);
+    t.cs_dtype = dtype_code(*c);
+    t.rot_dim = (int32_t)std::min<int64_t>(2 * c->size(1), 1 << 20);
+    if (const Tensor *p = given(positions)) {
+      check_same(rows, *p, "positions");
+      TORCH_CHECK(p->scalar_type() == at::kLong || p->scalar_type() == at::kInt, "kiv: positions must be int32 or int64");
+      const int64_t nl = (int64_t)lead.size();
+      TORCH_CHECK(p->dim() == nl || p->dim() == nl + 1, "kiv: positions must have ", nl, " dimensions, or an axis in front");
+      const int64_t o = p->dim() - nl;
+      for (int64_t i = 0; i < nl; ++i)
+        TORCH_CHECK(p->size(o + i) == lead[i], "kiv: positions do not match the tokens");
+      TORCH_CHECK(o == 0 || p->size(0) >= 1, "kiv: positions without an axis");
+      t.positions = p->data_ptr();
+      t.pos_is_i64 = p->scalar_type() == at::kLong;
+      t.axes = o ? (int32_t)p->size(0) : 1;
+      t.pos_stride_a = o ? p->stride(0) : 0;
+      t.pos_stride_b = nl == 2 ? p->stride(o) : 0;
+      t.pos_stride_t = p->stride(o + nl - 1);
+    }
+    if (const Tensor *x = given(pair_axes)) {
+      check_same(rows, *x, "pair_axes");
+      TORCH_CHECK(x->scalar_type() == at::kInt && x->dim() == 1 && x->is_contiguous() && x->size(0) == c->size(1),
+                  "kiv: pair_axes must be int32 [rot_dim / 2]");
+      t.pair_axes = x->data_ptr<int32_t>();
+    }
+    TORCH_CHECK(t.axes == 1 || t.pair_axes, "kiv: positions of several axes need pair_axes");
+    TORCH_CHECK(t.positions || rows_given || t.cs_rows == lead[0] * lead[lead.size() - 1],
+                "kiv: without positions, cos and sin need a row for each token");
+  } else {
+    TORCH_CHECK(!given(positions) && !given(pair_axes), "kiv: positions without cos and sin");
+  }
+  t.interleaved = interleaved;
+  t.norm = eps.has_value();
+  t.eps = (float)eps.value_or(0.0);
+  t.weight_offset = (float)weight_offset;
+  const Tensor *ws[2] = {given(q_weight), given(k_weight)};
+  for (int i = 0; i < 2; ++i) {
+    if (!ws[i]) continue;
+    TORCH_CHECK(t.norm, "kiv: a norm weight without eps");
+    check_same(rows, *ws[i], "norm weight");
+    TORCH_CHECK(ws[i]->dim() == 1 && ws[i]->size(0) == head_dim && ws[i]->is_contiguous(), "kiv: norm weights must be [head_dim]");
+    TORCH_CHECK(!(ws[0] && ws[1]) || ws[0]->scalar_type() == ws[1]->scalar_type(), "kiv: norm weights must have one dtype");
+    (i == 0 ? t.q_weight : t.k_weight) = ws[i]->data_ptr();
+    t.weight_dtype = dtype_code(*ws[i]);
+  }
+  return t;
+}
+
+kiv_rows make_rows(const Tensor &x, const char *what) {
+  TORCH_CHECK(x.dim() == 4 && x.stride(3) == 1, "kiv: ", what, " must be [B, H, Q, D] with a contiguous last dim");
+  return kiv_rows{x.data_ptr(), step(x, 0), step(x, 1), step(x, 2), (int32_t)x.size(1), 0};
+}
+
+void qk_norm_rope(const Tensor &q, const c10::optional<Tensor> &k, const c10::optional<Tensor> &cos,
+                  const c10::optional<Tensor> &sin, const c10::optional<Tensor> &positions,
+                  const c10::optional<Tensor> &pair_axes, bool interleaved, c10::optional<double> eps,
+                  const c10::optional<Tensor> &q_weight, const c10::optional<Tensor> &k_weight, double weight_offset,
+                  const Tensor &q_out, const c10::optional<Tensor> &k_out, const c10::optional<Tensor> &errors) {
+  c10::cuda::CUDAGuard g(q.device());
+  const kiv_rows qr = make_rows(q, "q"), qo = make_rows(q_out, "q_out");
+  check_same(q, q_out, "q_out");
+  TORCH_CHECK(q_out.sizes() == q.sizes() && q_out.scalar_type() == q.scalar_type(), "kiv: q_out must be like q");
+  const Tensor *kt = given(k), *kot = given(k_out);
+  TORCH_CHECK((kt != nullptr) == (kot != nullptr), "kiv: k and k_out come together");
+  kiv_rows kr = {}, ko = {};
+  if (kt) {
+    check_same(q, *kt, "k");
+    check_same(q, *kot, "k_out");
+    kr = make_rows(*kt, "k");
+    ko = make_rows(*kot, "k_out");
+    TORCH_CHECK(kot->sizes() == kt->sizes() && kt->scalar_type() == q.scalar_type() && kot->scalar_type() == q.scalar_type() &&
+                    kt->size(0) == q.size(0) && kt->size(2) == q.size(2) && kt->size(3) == q.size(3),
+                "kiv: k must match q in batch, tokens, head_dim and dtype, and k_out must be like k");
+  }
+  const int64_t lead[2] = {q.size(0), q.size(2)};
+  const kiv_turn t = make_turn(q, q.size(3), cos, sin, positions, pair_axes, interleaved, eps, q_weight, k_weight,
+                               weight_offset, lead, false);
+  TORCH_CHECK(q.size(0) * q.size(2) <= 0x7fffffff && q.size(3) <= (1 << 20), "kiv: too many tokens");
+  check(kiv_qk_norm_rope(dtype_code(q), (int32_t)q.size(0), (int32_t)q.size(2), (int32_t)q.size(3), &qr, kt ? &kr : nullptr,
+                         &qo, kt ? &ko : nullptr, &t, error_word(q, errors), stream_of(q)),
+        "qk_norm_rope");
+}
+
+kiv_paged make_paged(const Tensor &rows, const Tensor &k_pages, const Tensor &v_pages, const Tensor &table,
+                     const Tensor &seq_lens, const Tensor &q_starts, int64_t max_query_len,
+                     const c10::optional<Tensor> &errors) {
+  for (const Tensor *t : {&k_pages, &v_pages, &table, &seq_lens, &q_starts}) check_same(rows, *t, "the paged cache");
+  TORCH_CHECK(rows.dim() == 3 && rows.stride(2) == 1, "kiv: rows must be [tokens, heads, D] with a contiguous last dim");
+  TORCH_CHECK(k_pages.dim() == 4 && k_pages.stride(3) == 1 && v_pages.stride(3) == 1 && v_pages.sizes() == k_pages.sizes(),
+              "kiv: pages must both be [num_pages, Hkv, page_size, D] with a contiguous last dim");
+  TORCH_CHECK(k_pages.scalar_type() == rows.scalar_type() && v_pages.scalar_type() == rows.scalar_type(),
+              "kiv: rows and pages must have one dtype");
+  TORCH_CHECK(k_pages.size(3) == rows.size(2), "kiv: rows and pages must have one head_dim");
+  for (const Tensor *t : {&table, &seq_lens, &q_starts})
+    TORCH_CHECK(t->scalar_type() == at::kInt, "kiv: block_table, seq_lens and q_starts must be int32");
+  TORCH_CHECK(table.dim() == 2 && (table.size(1) <= 1 || table.stride(1) == 1), "kiv: block_table must be [batch, width]");
+  TORCH_CHECK(seq_lens.dim() == 1 && seq_lens.is_contiguous() && seq_lens.size(0) == table.size(0) && q_starts.dim() == 1 &&
+                  q_starts.is_contiguous() && q_starts.size(0) == table.size(0) + 1,
+              "kiv: seq_lens must be [batch] and q_starts [batch + 1]");
+  TORCH_CHECK(k_pages.size(1) <= 65536 && k_pages.size(2) <= (1 << 20) && k_pages.size(3) <= (1 << 20) &&
+                  table.size(0) <= (1 << 20) && max_query_len <= 0x7fffffff,
+              "kiv: paged cache too large");
+  kiv_paged p = {};
+  p.batch = (int32_t)table.size(0);
+  p.num_kv_heads = (int32_t)k_pages.size(1);
+  p.head_dim = (int32_t)k_pages.size(3);
+  p.page_size = (int32_t)k_pages.size(2);
+  p.dtype = dtype_code(rows);
+  p.max_query_len = (int32_t)max_query_len;
+  p.num_pages = k_pages.size(0);
+  p.k = ptr_or_null(k_pages);
+  p.v = ptr_or_null(v_pages);
+  p.k_stride_p = step(k_pages, 0);
+  p.k_stride_h = step(k_pages, 1);
+  p.k_stride_t = step(k_pages, 2);
+  p.v_stride_p = step(v_pages, 0);
+  p.v_stride_h = step(v_pages, 1);
+  p.v_stride_t = step(v_pages, 2);
+  p.block_table = static_cast<const int32_t *>(ptr_or_null(table));
+  p.table_stride = step(table, 0);
+  p.table_width = table.size(1);
+  p.seq_lens = static_cast<const int32_t *>(ptr_or_null(seq_lens));
+  p.q_starts = static_cast<const int32_t *>(ptr_or_null(q_starts));
+  p.num_tokens = rows.size(0);
+  p.errors = error_word(rows, errors);
+  return p;
+}
+
+void paged_append(const Tensor &k, const Tensor &v, const Tensor &k_pages, const Tensor &v_pages, const Tensor &table,
+                  const Tensor &seq_lens, const Tensor &q_starts, const c10::optional<Tensor> &cos,
+                  const c10::optional<Tensor> &sin, const c10::optional<Tensor> &positions,
+                  const c10::optional<Tensor> &pair_axes, bool interleaved, c10::optional<double> eps,
+                  const c10::optional<Tensor> &k_weight, double weight_offset, const c10::optional<Tensor> &errors) {
+  c10::cuda::CUDAGuard g(k.device());
+  check_same(k, v, "v");
+  const kiv_paged p = make_paged(k, k_pages, v_pages, table, seq_lens, q_starts, 0, errors);
+  TORCH_CHECK(v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type() && v.stride(2) == 1 && k.size(1) == p.num_kv_heads,
+              "kiv: new K/V rows must both be [tokens, Hkv, D]");
+  const int64_t lead[1] = {k.size(0)};
+  const kiv_turn t = make_turn(k, k.size(2), cos, sin, positions, pair_axes, interleaved, eps, c10::nullopt, k_weight,
+                               weight_offset, lead, true);
+  check(kiv_paged_append(&p, k.data_ptr(), step(k, 0), step(k, 1), v.data_ptr(), step(v, 0), step(v, 1), &t, stream_of(k)),
+        "paged_append");
+}
+
+void paged_attend(const Tensor &q, const Tensor &k_pages, const Tensor &v_pages, const Tensor &table, const Tensor &seq_lens,
+                  const Tensor &q_starts, double scaling, bool causal, int64_t window, double softcap, int64_t max_query_len,
+                  const Tensor &out, const c10::optional<Tensor> &lse, const c10::optional<Tensor> &errors) {
+  c10::cuda::CUDAGuard g(q.device());
+  const kiv_paged p = make_paged(q, k_pages, v_pages, table, seq_lens, q_starts, max_query_len, errors);
+  check_same(q, out, "out");
+  TORCH_CHECK(out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type() && out.stride(2) == 1, "kiv: out must be like q");
+  TORCH_CHECK(window >= 0 && window <= 0x7fffffff, "kiv: bad window");
+  kiv_paged_query d = {};
+  d.q = q.data_ptr();
+  d.stride_t = step(q, 0);
+  d.stride_h = step(q, 1);
+  d.out = out.data_ptr();
+  d.out_stride_t = step(out, 0);
+  d.out_stride_h = step(out, 1);
+  if (const Tensor *l = given(lse)) {
+    check_same(q, *l, "lse");
+    TORCH_CHECK(l->scalar_type() == at::kFloat && l->dim() == 2 && l->size(0) == q.size(0) && l->size(1) == q.size(1) && l->is_contiguous(),
+                "kiv: lse must be a contiguous float32 [tokens, Hq]");
+    d.lse = l->data_ptr<float>();
+  }
+  d.num_query_heads = (int32_t)q.size(1);
+  d.causal = causal;
+  d.window = (int32_t)window;
+  d.scaling = (float)scaling;
+  d.softcap = (float)softcap;
+  // scratch of this call alone, from the allocator of the stream (or graph) it runs in
+  const size_t bytes = kiv_paged_workspace_bytes(&p, &d);
+  Tensor ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
+  check(kiv_paged_attend(&p, &d, bytes ? ws.data_ptr() : nullptr, bytes, stream_of(q)), "paged_attend");
+}
+
 // ------------------------------------------------------------ shape queries
 // Workspace size and sub-buffer offsets: pure arithmetic on shapes (the data
 // pointers are stand-ins), so the same kernel serves real and fake tensors.
@@ -423,6 +637,17 @@ void attend_peers_meta(at::TensorList, at::IntArrayRef, const Tensor &, double, 
                        at::IntArrayRef, const Tensor &) {}
 void attend_exchange_merge_meta(at::TensorList, at::IntArrayRef, const Tensor &, double, int64_t, int64_t, double,
                                 const Tensor &, at::IntArrayRef, int64_t, int64_t, const Tensor &) {}
+void qk_norm_rope_meta(const Tensor &, const c10::optional<Tensor> &, const c10::optional<Tensor> &,
+                       const c10::optional<Tensor> &, const c10::optional<Tensor> &, const c10::optional<Tensor> &, bool,
+                       c10::optional<double>, const c10::optional<Tensor> &, const c10::optional<Tensor> &, double,
+                       const Tensor &, const c10::optional<Tensor> &, const c10::optional<Tensor> &) {}
+void paged_append_meta(const Tensor &, const Tensor &, const Tensor &, const Tensor &, const Tensor &, const Tensor &,
+                       const Tensor &, const c10::optional<Tensor> &, const c10::optional<Tensor> &,
+                       const c10::optional<Tensor> &, const c10::optional<Tensor> &, bool, c10::optional<double>,
+                       const c10::optional<Tensor> &, double, const c10::optional<Tensor> &) {}
+void paged_attend_meta(const Tensor &, const Tensor &, const Tensor &, const Tensor &, const Tensor &, const Tensor &,
+                       double, bool, int64_t, double, int64_t, const Tensor &, const c10::optional<Tensor> &,
+                       const c10::optional<Tensor> &) {}
 
 }  // namespace
 
@@ -470,6 +695,16 @@ TORCH_LIBRARY(kiv, m) {
   // every shard's cold tier; peer addresses as int[])
   m.def("attend_peers(Tensor(a!)[] store, int[] geom, " KIV_Q ", Tensor(b!) ws, Tensor sel, Tensor? mask_add, "
         "bool causal, int[] peer_k, int[] peer_v, Tensor(c!) out) -> ()");
+  // Rotation and paged cache (no reference counterpart: its caches are dense)
+  m.def("qk_norm_rope(Tensor q, Tensor? k, Tensor? cos, Tensor? sin, Tensor? positions, Tensor? pair_axes, "
+        "bool interleaved, float? eps, Tensor? q_weight, Tensor? k_weight, float weight_offset, Tensor(a!) q_out, "
+        "Tensor(b!)? k_out, Tensor(c!)? errors) -> ()");
+  m.def("paged_append(Tensor k, Tensor v, Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor block_table, Tensor seq_lens, "
+        "Tensor q_starts, Tensor? cos, Tensor? sin, Tensor? positions, Tensor? pair_axes, bool interleaved, float? eps, "
+        "Tensor? k_weight, float weight_offset, Tensor(c!)? errors) -> ()");
+  m.def("paged_attend(Tensor q, Tensor k_pages, Tensor v_pages, Tensor block_table, Tensor seq_lens, Tensor q_starts, "
+        "float scaling, bool causal, int window, float softcap, int max_query_len, Tensor(a!) out, Tensor(b!)? lse, "
+        "Tensor(c!)? errors) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(kiv, CUDA, m) {
@@ -490,6 +725,9 @@ TORCH_LIBRARY_IMPL(kiv, CUDA, m) {
   m.impl("attend_exchange_merge", &attend_exchange_merge);
   m.impl("fine_exchange_select", &fine_exchange_select);
   m.impl("attend_peers", &attend_peers);
+  m.impl("paged_attend", &paged_attend);
+  m.impl("paged_append", &paged_append);
+  m.impl("qk_norm_rope", &qk_norm_rope);
 }
 
 TORCH_LIBRARY_IMPL(kiv, Meta, m) {
@@ -510,6 +748,9 @@ TORCH_LIBRARY_IMPL(kiv, Meta, m) {
   m.impl("attend_exchange_merge", &attend_exchange_merge_meta);
   m.impl("fine_exchange_select", &fine_exchange_select_meta);
   m.impl("attend_peers", &attend_peers_meta);
+  m.impl("paged_attend", &paged_attend_meta);
+  m.impl("paged_append", &paged_append_meta);
+  m.impl("qk_norm_rope", &qk_norm_rope_meta);
 }
 
 TORCH_LIBRARY_IMPL(kiv, CompositeExplicitAutograd, m) { m.impl("workspace_layout", &workspace_layout); }

@@ -70,3 +70,5 @@ OP_NAMES = ("state_reset", "append_evict", "workspace_layout", "coarse_select", 
             "fine_topk", "fine_select", "fine_merge", "gather_rows", "attend", "attend_merge", "retrieve_attend",
             "coarse_exchange_merge", "fine_exchange_merge", "attend_exchange_merge", "fine_exchange_select",
             "attend_peers")
+# operators that take no store: rotation of queries and keys, and the paged cache (kiv_b200.paged)
+PAGED_OP_NAMES = ("qk_norm_rope", "paged_append", "paged_attend")
