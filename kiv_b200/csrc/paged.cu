@@ -90,11 +90,10 @@ __global__ void __launch_bounds__(CC_THREADS) paged_cc_kernel(const __grid_const
   float *sk = sq + R * ld, *sv = sk + CC_KEYS * ld, *sp = sv + CC_KEYS * ld;
   const int tr = threadIdx.x / 16, tc = threadIdx.x % 16;
   griddep_wait();
-  PagedSpot at = paged_locate<CC_THREADS>(p, blockIdx.x, gridDim.x, sm);
-  const int64_t end = (int64_t)(blockIdx.x + 1) * at.total / gridDim.x;
+  PagedSpot at = paged_locate<CC_THREADS>(p, sm);
   if (threadIdx.x == 0) p.cut[blockIdx.x].b = -1;
-  while (at.it.s.b >= 0 && at.unit < end) {
-    const PagedSegment g = paged_segment(p, at, end);
+  while (at.it.s.b >= 0 && at.unit < at.end) {
+    const PagedSegment g = paged_segment(p, at);
     const int kvh = at.hp / p.hs;
     int lo, hi;
     paged_range(p, at.it, at.rt, lo, hi);
@@ -281,7 +280,7 @@ __global__ void __launch_bounds__(CC_THREADS) paged_cc_kernel(const __grid_const
 constexpr int CB_WARPS = 8;
 
 template <typename T>
-__global__ void __launch_bounds__(CB_WARPS * 32) paged_combine_kernel(const __grid_constant__ PagedPlan p, int blocks) {
+__global__ void __launch_bounds__(CB_WARPS * 32) paged_combine_kernel(const __grid_constant__ PagedPlan p) {
   griddep_wait();
   const PagedCut cut = p.cut[blockIdx.x];
   if (cut.b < 0) return;
@@ -289,26 +288,16 @@ __global__ void __launch_bounds__(CB_WARPS * 32) paged_combine_kernel(const __gr
   const int slices = (D + 127) / 128;
   const PagedItems it = paged_items(p, cut.b);
   const int warp = (blockIdx.y * CB_WARPS + (threadIdx.x >> 5)), nwarps = gridDim.y * CB_WARPS;
-  // parts: slot 2c + 1, then slot 2c' of each later block whose stretch begins inside the item
+  // parts: slot 2c + 1, then slot 2c' of each later block c' whose stretch
+  // begins inside the item (c' N / G < end)
   const int c0 = blockIdx.x;
-  int last = c0;
-  {
-    // block c' takes part while its stretch begins before the item's end: c' N / G < end
-    int a = c0, z = blocks;            // a takes part, z does not
-    while (z - a > 1) {
-      const int mid = (a + z) / 2;
-      if ((int64_t)mid * cut.total / blocks < cut.end) a = mid; else z = mid;
-    }
-    last = a;
-  }
+  const int last = (int)((cut.end * cut.blocks - 1) / cut.total);
   for (int x = warp; x < p.tpt * p.grp * slices; x += nwarps) {
     const int r = x / slices, col = (x % slices) * 128 + 4 * lane;
     int i, head;
     if (!paged_row(p, it, cut.hp, cut.rt, r, i, head)) continue;
     float mx = -INFINITY;
     for (int c = c0 + lane; c <= last; c += 32) {
-      // a block with an empty stretch (fewer tiles than blocks) left nothing
-      if ((int64_t)c * cut.total / blocks == (int64_t)(c + 1) * cut.total / blocks) continue;
       mx = fmaxf(mx, paged_part(p, 2 * (int64_t)c + (c == c0), r)[D]);
     }
 #pragma unroll
@@ -318,7 +307,6 @@ __global__ void __launch_bounds__(CB_WARPS * 32) paged_combine_kernel(const __gr
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
     for (int c = c0; c <= last; ++c) {
-      if ((int64_t)c * cut.total / blocks == (int64_t)(c + 1) * cut.total / blocks) continue;
       const float *src = paged_part(p, 2 * (int64_t)c + (c == c0), r);
       const float w = exp2f((src[D] - ms) * 1.44269504f);
       l = fmaf(src[D + 1], w, l);
@@ -348,9 +336,9 @@ kiv_status launch_paged_combine(const PagedPlan &p, int blocks, cudaStream_t s) 
   const int y = (int)std::min<int64_t>(ceil_div((int64_t)p.tpt * p.grp * slices, CB_WARPS), 8);
   const dim3 grid((unsigned)blocks, (unsigned)y), block(CB_WARPS * 32);
   cudaError_t e;
-  if (p.pc.dtype == KIV_DTYPE_F32) e = launch_pdl(paged_combine_kernel<float>, grid, block, 0, s, 1, p, blocks);
-  else if (p.pc.dtype == KIV_DTYPE_BF16) e = launch_pdl(paged_combine_kernel<__nv_bfloat16>, grid, block, 0, s, 1, p, blocks);
-  else e = launch_pdl(paged_combine_kernel<__half>, grid, block, 0, s, 1, p, blocks);
+  if (p.pc.dtype == KIV_DTYPE_F32) e = launch_pdl(paged_combine_kernel<float>, grid, block, 0, s, 1, p);
+  else if (p.pc.dtype == KIV_DTYPE_BF16) e = launch_pdl(paged_combine_kernel<__nv_bfloat16>, grid, block, 0, s, 1, p);
+  else e = launch_pdl(paged_combine_kernel<__half>, grid, block, 0, s, 1, p);
   return cuda_status(e, "paged_combine");
 }
 
@@ -366,12 +354,15 @@ static PagedPlan make_plan(const kiv_paged *pc, const kiv_paged_query *q, int ro
   p.tpt = rows / p.grp;
   p.kt = kt;
   p.rows = rows;
-  p.min_rows = 0;
-  p.max_rows = 0x7fffffff;
+  p.min_tokens = 0;
+  p.max_tokens = 0x7fffffff;
   return p;
 }
 
+enum PagedKernel { PAGED_CC, PAGED_MMA, PAGED_TC };
+
 struct PagedCall {
+  PagedKernel kernel;
   PagedPlan p;
   int blocks;
   size_t bytes;        // of its workspace
@@ -383,21 +374,54 @@ static void size_call(PagedCall &c) {
   c.bytes = c.cut_offset + (size_t)align_up((int64_t)c.blocks * sizeof(PagedCut), 256);
 }
 
-// rows a sequence of the largest (or, unknown, the average) length brings per key head
-static int64_t likely_rows(const kiv_paged *pc, const kiv_paged_query *q) {
-  const int64_t per = q->num_query_heads / pc->num_kv_heads;
-  const int64_t n = pc->max_query_len > 0 ? pc->max_query_len : ceil_div(pc->num_tokens, std::max(1, pc->batch));
-  return per * n;
-}
+// Rows per key head from which a sequence's chunk goes to tcgen05
+constexpr int TC_ROWS = 65;
 
-static PagedCall plan_cc(const kiv_paged *pc, const kiv_paged_query *q) {
-  PagedCall c;
-  const int rows = likely_rows(pc, q) <= 16 ? 16 : 64;
-  c.p = make_plan(pc, q, rows, CC_KEYS);
-  const size_t smem = rows == 16 ? cc_smem<16>(pc->head_dim) : cc_smem<64>(pc->head_dim);
-  c.blocks = sm_count() * (int)std::max<size_t>(1, std::min<size_t>(4, (220 * 1024) / (smem + 2048)));
-  size_call(c);
-  return c;
+// The kernels of a call (one or two) and their tilings.  The lengths are on
+// the device, so the host goes by what it knows: the number of rows, and
+// max_query_len.  Where that leaves both kinds of sequences possible, both
+// kernels run and each takes its own sequences.
+static int plan_calls(const kiv_paged *pc, const kiv_paged_query *q, PagedCall (&c)[2]) {
+  const int D = pc->head_dim;
+  const int64_t per = q->num_query_heads / pc->num_kv_heads, T = pc->num_tokens, B = std::max(1, pc->batch);
+  const int64_t most = std::min<int64_t>(T, pc->max_query_len > 0 ? pc->max_query_len : T);   // tokens of one sequence
+  const int64_t mean = ceil_div(T, B);
+  const int64_t likely = per * std::min(most, pc->max_query_len > 0 ? most : mean);
+  if (!paged_mma_head(pc->dtype, D)) {
+    const int rows = likely <= 16 ? 16 : 64;
+    c[0].kernel = PAGED_CC;
+    c[0].p = make_plan(pc, q, rows, CC_KEYS);
+    const size_t smem = rows == 16 ? cc_smem<16>(D) : cc_smem<64>(D);
+    c[0].blocks = sm_count() * (int)std::max<size_t>(1, std::min<size_t>(4, (220 * 1024) / (smem + 2048)));
+    size_call(c[0]);
+    return 1;
+  }
+  // most * B == T: every sequence has `most` new tokens.  T <= B: single tokens.
+  const bool tc = paged_tc_eligible(pc, q);
+  const bool only_small = !tc || per * most < TC_ROWS || (T <= B && pc->max_query_len == 0);
+  const bool only_large = !only_small && most * B == T;
+  int n = 0;
+  if (!only_large) {
+    PagedCall &m = c[n++];
+    const int64_t at = only_small ? likely : per;
+    const int rows = at <= 16 ? 16 : at <= 32 ? 32 : 64;
+    m.kernel = PAGED_MMA;
+    m.p = make_plan(pc, q, rows, 64);
+    if (!only_small) m.p.max_tokens = (int)((TC_ROWS - 1) / per);
+    m.blocks = paged_mma_blocks(D, rows);
+    size_call(m);
+  }
+  if (!only_small) {
+    PagedCall &t = c[n++];
+    t.kernel = PAGED_TC;
+    t.p = make_plan(pc, q, 128, 128);
+    t.p.tpt *= 2;
+    t.p.rows = 256;
+    if (!only_large) t.p.min_tokens = (int)((TC_ROWS - 1) / per) + 1;
+    t.blocks = sm_count();
+    size_call(t);
+  }
+  return n;
 }
 
 template <typename T, int R, int DM>
@@ -416,9 +440,11 @@ static cudaError_t launch_cc_r(const PagedCall &c, cudaStream_t s) {
   return c.p.rows == 16 ? launch_cc_d<T, 16>(c, s) : launch_cc_d<T, 64>(c, s);
 }
 
-static kiv_status run_cc(PagedCall c, char *ws, cudaStream_t s) {
+static kiv_status run_call(PagedCall c, char *ws, cudaStream_t s) {
   c.p.part = reinterpret_cast<float *>(ws);
   c.p.cut = reinterpret_cast<PagedCut *>(ws + c.cut_offset);
+  if (c.kernel == PAGED_MMA) return launch_paged_mma(c.p, c.blocks, s);
+  if (c.kernel == PAGED_TC) return launch_paged_tc(c.p, c.blocks, s);
   cudaError_t e;
   if (c.p.pc.dtype == KIV_DTYPE_F32) e = launch_cc_r<float>(c, s);
   else if (c.p.pc.dtype == KIV_DTYPE_BF16) e = launch_cc_r<__nv_bfloat16>(c, s);
@@ -435,19 +461,23 @@ extern "C" {
 
 size_t kiv_paged_workspace_bytes(const kiv_paged *pc, const kiv_paged_query *q) {
   if (check_paged(pc) != KIV_OK || !q || q->num_query_heads < 1 || q->num_query_heads % pc->num_kv_heads || pc->head_dim > 256) return 0;
-  return plan_cc(pc, q).bytes;
+  PagedCall c[2];
+  return plan_calls(pc, q, c) == 1 ? c[0].bytes : c[0].bytes + c[1].bytes;
 }
 
 kiv_status kiv_paged_attend(const kiv_paged *pc, const kiv_paged_query *q, void *ws, size_t ws_bytes, void *stream) {
   KIV_CHECK(check_paged(pc));
   KIV_CHECK(check_paged_query(pc, q));
   if (pc->num_tokens == 0 || pc->batch == 0) return KIV_OK;
-  const PagedCall c = plan_cc(pc, q);
-  if (!ws || ws_bytes < c.bytes || (reinterpret_cast<uintptr_t>(ws) & 255)) {
-    set_error("workspace too small or misaligned (%zu < %zu)", ws_bytes, c.bytes);
+  PagedCall c[2];
+  const int n = plan_calls(pc, q, c);
+  const size_t need = n == 1 ? c[0].bytes : c[0].bytes + c[1].bytes;
+  if (!ws || ws_bytes < need || (reinterpret_cast<uintptr_t>(ws) & 255)) {
+    set_error("workspace too small or misaligned (%zu < %zu)", ws_bytes, need);
     return KIV_ERR_CAPACITY;
   }
-  return run_cc(c, static_cast<char *>(ws), (cudaStream_t)stream);
+  KIV_CHECK(run_call(c[0], static_cast<char *>(ws), (cudaStream_t)stream));
+  return n == 1 ? KIV_OK : run_call(c[1], static_cast<char *>(ws) + c[0].bytes, (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -67,8 +67,9 @@ __device__ __forceinline__ PagedSeq paged_find_seq(const kiv_paged &pc, int64_t 
 // are more of them than a tile has rows).  Its work is the tiles of `kt` keys
 // that some row of it sees.  The items of the batch, in the order (sequence,
 // head part, row tile), make one line of tiles, and block c of G takes the
-// tiles [c N / G, (c + 1) N / G) of it: every block streams the same number
-// of key tiles (within one), whatever the lengths.  An item inside one block
+// tiles [c N / G, (c + 1) N / G) of it (G at most N: the other blocks leave):
+// every block streams the same number of key tiles (within one), whatever the
+// lengths.  An item inside one block
 // is finished there; one that blocks share leaves its parts (running maximum,
 // sum, unscaled output) in the workspace, at most two per block -- slot 2c for
 // an item that began in an earlier block, slot 2c + 1 for one that began in
@@ -86,7 +87,7 @@ struct PagedPlan {
   int tpt;       // tokens per row tile
   int kt;        // keys per key tile
   int rows;      // rows per part in the workspace: tpt * grp <= rows
-  int min_rows, max_rows;   // takes the sequences with min_rows <= grp * n <= max_rows
+  int min_tokens, max_tokens;   // takes the sequences whose new tokens' count is in this range
   float *part;   // [2 * G][rows][D + 2 (rounded to 4)]
   struct PagedCut *cut;     // [G]
 };
@@ -95,6 +96,7 @@ struct PagedPlan {
 struct PagedCut {
   int32_t b, hp, rt, pad;
   int64_t end, total;       // the place past the item's last tile; N
+  int64_t blocks;           // blocks that took part
 };
 
 __host__ __device__ inline int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
@@ -116,6 +118,16 @@ __host__ __device__ inline int64_t floor_sum(int64_t n, int64_t m, int64_t a, in
   return ans;
 }
 
+kiv_status launch_paged_combine(const PagedPlan &p, int blocks, cudaStream_t s);
+// few rows per key head, 16-bit rows (paged_mma.cu); plan rows 16, 32 or 64, kt 64
+bool paged_mma_head(int dtype, int D);
+int paged_mma_blocks(int D, int rows);
+kiv_status launch_paged_mma(const PagedPlan &p, int blocks, cudaStream_t s);
+
+// chunks, 16-bit rows, tcgen05 (paged_tc.cu); plan rows 256, kt 128, whole tokens per 128 rows
+bool paged_tc_eligible(const kiv_paged *pc, const kiv_paged_query *q);
+kiv_status launch_paged_tc(const PagedPlan &p, int blocks, cudaStream_t s);
+
 struct PagedItems {      // the items of one sequence
   PagedSeq s;
   int nrt;               // row tiles (0: none of this kernel's)
@@ -125,8 +137,7 @@ struct PagedItems {      // the items of one sequence
 __device__ __forceinline__ PagedItems paged_items(const PagedPlan &p, int b) {
   PagedItems it;
   it.s = paged_seq(p.pc, b);
-  const int64_t rows = (int64_t)it.s.n * p.grp;
-  it.nrt = it.s.n > 0 && rows >= p.min_rows && rows <= p.max_rows ? (it.s.n + p.tpt - 1) / p.tpt : 0;
+  it.nrt = it.s.n > 0 && it.s.n >= p.min_tokens && it.s.n <= p.max_tokens ? (it.s.n + p.tpt - 1) / p.tpt : 0;
   it.base = p.q.causal ? it.s.len - it.s.n : it.s.len;
   return it;
 }
@@ -181,13 +192,15 @@ struct PagedSpot {       // a place on the line of tiles
   int rt;
   int64_t off;           // tiles into the item
   int64_t total;         // N
+  int64_t blocks;        // G
   int64_t unit;          // the place itself
+  int64_t end;           // where the block's stretch ends
 };
 
-// Place of unit (num N / den) on the line, for the whole block.  `sm`: shared,
-// 40 words of 8 bytes.  b = -1 in the result: at or past the end.
+// The stretch of this block (blockIdx.x), found by the whole block.  `sm`:
+// shared, 40 words of 8 bytes.  b = -1 in the result: nothing to do.
 template <int NT>
-__device__ __forceinline__ PagedSpot paged_locate(const PagedPlan &p, int64_t num, int64_t den, int64_t *sm) {
+__device__ __forceinline__ PagedSpot paged_locate(const PagedPlan &p, int64_t *sm) {
   const int H = p.pc.num_kv_heads * p.hs;
   const int per = (p.pc.batch + NT - 1) / NT;
   const int b0 = threadIdx.x * per, b1 = min(b0 + per, p.pc.batch);
@@ -214,7 +227,8 @@ __device__ __forceinline__ PagedSpot paged_locate(const PagedPlan &p, int64_t nu
     if (w < warp) before += sm[w];
     total += sm[w];
   }
-  const int64_t unit = num * total / den;   // below 2^63: N counts tiles, num blocks
+  const int64_t G = min((int64_t)gridDim.x, total), c = blockIdx.x;
+  const int64_t unit = c < G ? c * total / G : total;   // below 2^63: N counts tiles, c blocks
   int64_t at = unit - (before + inc - mine);
   if (at >= 0 && at < mine) {
     for (int b = b0; b < b1; ++b) {
@@ -231,7 +245,9 @@ __device__ __forceinline__ PagedSpot paged_locate(const PagedPlan &p, int64_t nu
   __syncthreads();
   PagedSpot r;
   r.total = total;
+  r.blocks = G;
   r.unit = unit;
+  r.end = c < G ? (c + 1) * total / G : total;
   r.hp = r.rt = 0;
   r.off = 0;
   const int b = (int)sm[32];
@@ -269,17 +285,17 @@ __device__ __forceinline__ void paged_next(const PagedPlan &p, PagedSpot &s) {
   s.it.s.b = -1;
 }
 
-// One segment of a block's stretch [at.unit, end): the item's tiles [t0, t1)
+// One segment of a block's stretch [at.unit, at.end): the item's tiles [t0, t1)
 struct PagedSegment {
   int t0, t1;
   bool head, tail;       // the item began in an earlier block / goes on in a later one
 };
 
-__device__ __forceinline__ PagedSegment paged_segment(const PagedPlan &p, const PagedSpot &at, int64_t end) {
+__device__ __forceinline__ PagedSegment paged_segment(const PagedPlan &p, const PagedSpot &at) {
   PagedSegment g;
   const int nt = paged_tiles(p, at.it, at.rt);
   g.t0 = (int)at.off;
-  g.t1 = (int)min((int64_t)nt, at.off + (end - at.unit));
+  g.t1 = (int)min((int64_t)nt, at.off + (at.end - at.unit));
   g.head = g.t0 > 0;
   g.tail = g.t1 < nt;
   return g;
@@ -295,6 +311,7 @@ __device__ __forceinline__ void paged_record(const PagedPlan &p, int c, const Pa
     r.rt = at.rt;
     r.end = at.unit - at.off + paged_tiles(p, at.it, at.rt);
     r.total = at.total;
+    r.blocks = at.blocks;
   }
   p.cut[c] = r;
 }
