@@ -9,7 +9,7 @@
 // (`tps` = 128 / heads whole tokens per tile).  Warp roles:
 //   warp 8   TMA: the query tiles, then K and V tiles of 128 keys through a
 //            ring, one box of `br` rows per page piece;
-//   warp 9   MMA: S_i(j+1) right behind O_i += P_i(j) V(j) for i = 0, 1;
+//   warps 9, 10  MMA of row tile 0 and 1: O += P(j) V(j), then S(j+1);
 //   warps 0-3 and 4-7: softmax of row tile 0 and 1, a thread per row.
 // While one row tile's softmax runs, the tensor cores work on the other's
 // products, so both are kept busy: per tile pair the tensor cores need 4 x 512
@@ -24,7 +24,7 @@
 //
 // Key tiles that hold the end of a sequence (or keys before a window) may hold
 // anything in the dead rows, NaN too: scores there are replaced, not added to,
-// and the MMA warp clears the dead V rows before the product.
+// and the softmax groups clear the dead V rows before their products.
 #include <algorithm>
 
 #include "internal.h"
@@ -35,7 +35,10 @@ namespace kiv {
 
 constexpr int PT_KEYS = 128;
 constexpr int PT_ROWS = 128;                   // of one row tile
-constexpr int PT_THREADS = 320;
+constexpr int PT_THREADS = 384;                // three warpgroups: two of softmax, one with the TMA and the MMA warp
+// registers per thread: 168 at launch, (2 x 208 + 88) x 128 = 168 x 384 after the split
+constexpr int PT_REGS_SOFTMAX = 208, PT_REGS_OTHER = 88;
+constexpr int PT_HEAD = 96;                    // keys of a tile whose P V product begins before the rest of P is there
 constexpr float PT_LAZY = 8.f;                 // growth (log2) that a row's reference may lag behind
 
 struct PagedTcGeom {
@@ -113,6 +116,12 @@ __device__ __forceinline__ void wait_ld32(uint32_t *r) {
                :
                : "memory");
 }
+__device__ __forceinline__ void wait_ld16(uint32_t *r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+}
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, int32_t x, int32_t y, int32_t z, uint64_t *bar) {
   asm volatile(
@@ -129,6 +138,13 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// one lane of the (converged) warp
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+  return p != 0;
+}
+
 template <bool BF>
 __device__ __forceinline__ uint32_t pt_pack(float x, float y) {
   if constexpr (BF) {
@@ -140,30 +156,17 @@ __device__ __forceinline__ uint32_t pt_pack(float x, float y) {
   }
 }
 
-// Walks the segments of a block's stretch, the same for every warp role.
-struct PtWalk {
-  PagedSpot at;
-  PagedSegment sg;
-  int lo, hi;
-  int64_t j00;
-  int ntile, nsub;
-  __device__ __forceinline__ bool live() const { return at.it.s.b >= 0 && at.unit < at.end; }
-  __device__ __forceinline__ void open(const PagedPlan &p, int tps) {
-    sg = paged_segment(p, at);
-    paged_range(p, at.it, at.rt, lo, hi);
-    hi = min(hi, at.it.s.len);
-    j00 = ((int64_t)lo / PT_KEYS + sg.t0) * PT_KEYS;
-    ntile = sg.t1 - sg.t0;
-    nsub = at.it.s.n - at.rt * p.tpt > tps ? 2 : 1;
-  }
-  __device__ __forceinline__ void next(const PagedPlan &p) {
-    at.unit += ntile;
-    if (sg.tail) {
-      at.it.s.b = -1;
-      return;
-    }
-    paged_next(p, at);
-  }
+// One segment of the block's stretch, as the TMA warp tells the others.
+struct PtSeg {
+  int ntile;       // 0: no more
+  int nsub;        // row tiles that have tokens
+  int lo, hi;      // live keys
+  int64_t j00;     // first key of its first key tile
+  int64_t q0;      // packed row of token 0 of the item's first row tile
+  int tok;         // tokens from there on
+  int base;        // place of that token (causal), or the length
+  int head0, heads;   // its query heads
+  int part;        // workspace slot, or -1: the rows are finished here
 };
 
 template <bool BF, int D>
@@ -174,23 +177,26 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
   using T = typename std::conditional<BF, __nv_bfloat16, __half>::type;
   constexpr int SLOTS = S::SLOTS;
   extern __shared__ uint8_t pt_dyn[];
-  __shared__ uint64_t q_full, q_empty, kv_full[SLOTS], kv_empty[SLOTS], s_full[2], p_full[2], o_full[2];
+  __shared__ uint64_t q_full, q_empty, kv_full[SLOTS], kv_empty[SLOTS], s_full[2], p_full[2], p_tail[2], o_full[2];
   __shared__ int64_t sm[40];
   __shared__ uint32_t s_tmem;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  __shared__ PtSeg seg[2];
+  // broadcast: the compiler then knows that a role's control flow is the warp's
+  const int warp = __shfl_sync(KIV_FULL_MASK, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   uint8_t *smem = pt_dyn + ((1024 - (smem_u32(pt_dyn) & 1023)) & 1023);
   uint8_t *qmem = smem, *ring = smem + 2 * S::TILE;
 
   if (threadIdx.x == 0) {
     mbar_init(&q_full, 1);
-    mbar_init(&q_empty, 1);
+    mbar_init(&q_empty, 10);                   // each row tile's last scores; the softmax warps have read `seg`
     for (int i = 0; i < SLOTS; ++i) {
       mbar_init(&kv_full[i], 1);
-      mbar_init(&kv_empty[i], 1);
+      mbar_init(&kv_empty[i], 2);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
+      mbar_init(&p_tail[i], 4);
       mbar_init(&o_full[i], 1);
     }
     mbar_fence_init();
@@ -212,38 +218,62 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
   tc::fence_after_sync();
   const uint32_t tmem = s_tmem;
   griddep_wait();
-  PtWalk w;
-  w.at = paged_locate<PT_THREADS>(p, sm);
+  PagedSpot at = paged_locate<PT_THREADS>(p, sm);
   if (threadIdx.x == 0) p.cut[blockIdx.x].b = -1;
   bool ok = true;
   const int rows = g.tps * p.grp;              // of a row tile
-  const int per = p.q.num_query_heads / p.pc.num_kv_heads;
-
-  if (warp == 8) {
+  if (warp >= 8) {
+   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PT_REGS_OTHER));
+   if (warp == 8) {
     // ------------------------------------------------ TMA
     uint32_t n = 0, items = 0;
-    for (; w.live(); w.next(p), ++items) {
-      w.open(p, g.tps);
-      const int kvh = w.at.hp / p.hs, head0 = kvh * per + (w.at.hp % p.hs) * p.grp;
-      if (lane == 0) {
-        if (!w.sg.head) paged_check_lens(p.pc, w.at.it.s);
-        if (w.sg.tail) paged_record(p, blockIdx.x, w.at, w.sg);
-        if (items > 0 && ok && !mbar_wait_bounded(&q_empty, (items - 1) & 1)) ok = false;
-        mbar_arrive_tx(&q_full, (uint32_t)w.nsub * rows * D * 2);
-        for (int i = 0; i < w.nsub; ++i)
-          for (int c = 0; c < S::NB; ++c)
-            tc::tma_load_3d(qmem + i * S::TILE + c * (PT_ROWS * S::BOXB), &qmap, c * S::BOX, head0,
-                            (int32_t)(w.at.it.s.q0 + (int64_t)w.at.rt * p.tpt + i * g.tps), &q_full);
+    const int per = p.q.num_query_heads / p.pc.num_kv_heads;
+    for (;; ++items) {
+      const bool live = at.it.s.b >= 0 && at.unit < at.end;
+      PtSeg sg = {};
+      PagedSegment cut = {};
+      int kvh = 0;
+      if (live) {
+        cut = paged_segment(p, at);
+        paged_range(p, at.it, at.rt, sg.lo, sg.hi);
+        sg.hi = min(sg.hi, at.it.s.len);
+        sg.j00 = ((int64_t)sg.lo / PT_KEYS + cut.t0) * PT_KEYS;
+        sg.ntile = cut.t1 - cut.t0;
+        const int first = at.rt * p.tpt;
+        sg.q0 = at.it.s.q0 + first;
+        sg.tok = min(at.it.s.n - first, p.tpt);
+        sg.nsub = sg.tok > g.tps ? 2 : 1;
+        sg.base = p.q.causal ? at.it.base + first : at.it.s.len;
+        kvh = at.hp / p.hs;
+        sg.head0 = kvh * per + (at.hp % p.hs) * p.grp;
+        sg.heads = min(p.grp, per - (at.hp % p.hs) * p.grp);
+        sg.part = cut.head ? 2 * (int)blockIdx.x : cut.tail ? 2 * (int)blockIdx.x + 1 : -1;
       }
+      if (items > 0 && ok && !mbar_wait_bounded(&q_empty, (items - 1) & 1)) ok = false;
+      if (lane == 0) {
+        seg[items & 1] = sg;
+        if (!live) {
+          mbar_arrive(&q_full);
+        } else {
+          if (!cut.head) paged_check_lens(p.pc, at.it.s);
+          if (cut.tail) paged_record(p, blockIdx.x, at, cut);
+          mbar_arrive_tx(&q_full, (uint32_t)sg.nsub * rows * D * 2);
+          for (int i = 0; i < sg.nsub; ++i)
+            for (int c = 0; c < S::NB; ++c)
+              tc::tma_load_3d(qmem + i * S::TILE + c * (PT_ROWS * S::BOXB), &qmap, c * S::BOX, sg.head0,
+                              (int32_t)(sg.q0 + i * g.tps), &q_full);
+        }
+      }
+      if (!live) break;
       __syncwarp();
       // lane l brings rows [l br, (l + 1) br) of every tile
       const int nbox = PT_KEYS / g.br;
-      const int32_t *table = p.pc.block_table + w.at.it.s.b * p.pc.table_stride;
+      const int32_t *table = p.pc.block_table + at.it.s.b * p.pc.table_stride;
       auto lookup = [&](int t, int32_t &page, int32_t &row) {
         page = -1;                             // outside: the box reads as zeros
         row = 0;
-        const int64_t j = w.j00 + (int64_t)t * PT_KEYS + lane * g.br;
-        if (t < w.ntile && lane < nbox && j < w.hi && j + g.br > w.lo) {
+        const int64_t j = sg.j00 + (int64_t)t * PT_KEYS + lane * g.br;
+        if (t < sg.ntile && lane < nbox && j < sg.hi && j + g.br > sg.lo) {
           const uint32_t pg = (uint32_t)j / (uint32_t)p.pc.page_size;
           row = (int32_t)((uint32_t)j - pg * (uint32_t)p.pc.page_size);
           page = table[pg];
@@ -255,7 +285,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
       };
       int32_t page, row;
       lookup(0, page, row);
-      for (int t = 0; t < w.ntile; ++t) {
+      for (int t = 0; t < sg.ntile; ++t) {
         const int32_t pg = page, rw = row;
         lookup(t + 1, page, row);
         for (int kv = 0; kv < 2; ++kv, ++n) {
@@ -269,136 +299,170 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
                               rw, kvh, pg, &kv_full[s]);
         }
       }
+      at.unit += sg.ntile;
+      if (cut.tail)
+        at.it.s.b = -1;
+      else
+        paged_next(p, at);
     }
-  } else if (warp == 9) {
-    // ------------------------------------------------ MMA
-    const uint32_t id_s = tc::idesc_f16(BF, PT_ROWS, PT_KEYS);
-    const uint32_t id_o = tc::idesc_f16(BF, PT_ROWS, D) | (1u << 16);     // B is MN-major
-    uint32_t n = 0, items = 0, tiles[2] = {0, 0};
+   } else if (warp < 11) {
+    // ------------------------------------------------ MMA of row tile i
+    // The tensor pipe takes few products ahead, so what an issuing warp does
+    // between them is lost time; with a warp per row tile, one's waits pass
+    // under the other's products.  The whole warp walks the loop and one lane
+    // issues, so that descriptors stay in uniform registers.
+    const int i = warp - 9;
+    constexpr uint32_t id_s = tc::idesc_f16(BF, PT_ROWS, PT_KEYS);
+    constexpr uint32_t id_o = tc::idesc_f16(BF, PT_ROWS, D) | (1u << 16);     // B is MN-major
+    constexpr uint32_t TILE16 = S::TILE >> 4;
+    const uint64_t qd = (S::BOX == 64 ? tc::sdesc_k128(smem_u32(qmem)) : tc::sdesc_k64(smem_u32(qmem))) + (uint32_t)i * TILE16;
+    const uint64_t kd = S::BOX == 64 ? tc::sdesc_k128(smem_u32(ring)) : tc::sdesc_k64(smem_u32(ring));
+    const uint64_t vd = tc::sdesc_mn<S::BOXB>(smem_u32(ring), PT_KEYS * S::BOXB);
+    const uint32_t ts = tmem + i * PT_KEYS, to = tmem + 2 * PT_KEYS + i * D;
+    uint32_t slot = 0, phase = 0;              // of the next K or V tile
+    uint32_t tiles = 0;
+    const bool leader = elect_one();
     auto wait = [&](uint64_t *bar, uint32_t parity) {
       if (ok && !mbar_wait_bounded(bar, parity)) ok = false;
-      tc::fence_after_sync();
     };
-    auto scores = [&](int i, uint32_t slot) {
-      if (lane != 0) return;
-      const uint32_t a0 = smem_u32(qmem + i * S::TILE), b0 = smem_u32(ring + slot * S::TILE);
+    auto bump = [&]() {
+      if (++slot == SLOTS) {
+        slot = 0;
+        phase ^= 1;
+      }
+    };
+    auto scores = [&]() {
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
-        const uint32_t off = (uint32_t)(k * 16 / S::BOX) * (PT_ROWS * S::BOXB) + (uint32_t)(k * 16 % S::BOX) * 2;
-        const uint64_t ad = S::BOX == 64 ? tc::sdesc_k128(a0 + off) : tc::sdesc_k64(a0 + off);
-        const uint64_t bd = S::BOX == 64 ? tc::sdesc_k128(b0 + off) : tc::sdesc_k64(b0 + off);
-        tc::mma_f16(tmem + i * PT_KEYS, ad, bd, id_s, k > 0 ? 1u : 0u);
+        const uint32_t off = ((uint32_t)(k * 16 / S::BOX) * (PT_ROWS * S::BOXB) + (uint32_t)(k * 16 % S::BOX) * 2) >> 4;
+        tc::mma_f16(ts, qd + off, kd + slot * TILE16 + off, id_s, k > 0 ? 1u : 0u);
       }
       tc::commit(&s_full[i]);
+      tc::commit(&kv_empty[slot]);
     };
-    for (; w.live(); w.next(p), ++items) {
-      w.open(p, g.tps);
+    for (uint32_t items = 0;; ++items) {
       wait(&q_full, items & 1);
-      wait(&kv_full[n % SLOTS], (n / SLOTS) & 1);
-      for (int i = 0; i < w.nsub; ++i) scores(i, n % SLOTS);
-      if (lane == 0) {
-        tc::commit(&kv_empty[n % SLOTS]);
-        if (w.ntile == 1) tc::commit(&q_empty);
+      const int ntile = __shfl_sync(KIV_FULL_MASK, ok ? seg[items & 1].ntile : 0, 0);
+      const int nsub = __shfl_sync(KIV_FULL_MASK, seg[items & 1].nsub, 0);
+      if (ntile == 0) break;
+      if (i >= nsub) {                         // no such row tile: only pass the ring on
+        if (leader) mbar_arrive(&q_empty);
+        for (int t = 0; t < 2 * ntile; ++t) {
+          wait(&kv_full[slot], phase);
+          __syncwarp();
+          if (leader) mbar_arrive(&kv_empty[slot]);
+          bump();
+        }
+        continue;
       }
-      for (int t = 0; t < w.ntile; ++t, n += 2) {
-        const uint32_t vs = (n + 1) % SLOTS, ks = (n + 2) % SLOTS;
-        wait(&kv_full[vs], ((n + 1) / SLOTS) & 1);
-        // dead rows of the V tile
-        const int64_t j0 = w.j00 + (int64_t)t * PT_KEYS;
-        const int dl = (int)max((int64_t)0, w.lo - j0), dh = (int)min((int64_t)PT_KEYS, w.hi - j0);
-        if (dl > 0 || dh < PT_KEYS) {
-          for (int x = lane; x < PT_KEYS * S::NB * (S::BOXB / 16); x += 32) {
-            const int r = x / (S::NB * (S::BOXB / 16)), c = x % (S::NB * (S::BOXB / 16));
-            if (r < dl || r >= dh)
-              *reinterpret_cast<uint4 *>(ring + vs * S::TILE + (c / (S::BOXB / 16)) * (PT_KEYS * S::BOXB) + r * S::BOXB +
-                                         (c % (S::BOXB / 16)) * 16) = make_uint4(0, 0, 0, 0);
-          }
-          tc::fence_proxy_async_smem();
-          __syncwarp();
-        }
-        const bool more = t + 1 < w.ntile;
-        for (int i = 0; i < w.nsub; ++i) {
-          wait(&p_full[i], tiles[i] & 1);
-          ++tiles[i];
-          if (lane == 0) {
-            const uint32_t b0 = smem_u32(ring + vs * S::TILE);
+      wait(&kv_full[slot], phase);
+      tc::fence_after_sync();
+      if (leader) {
+        scores();
+        if (ntile == 1) tc::commit(&q_empty);
+      }
+      bump();
+      for (int t = 0; t < ntile; ++t, ++tiles) {
+        const bool more = t + 1 < ntile;
+        const uint32_t vs = slot;
+        wait(&kv_full[vs], phase);
+        bump();
+        if (more) wait(&kv_full[slot], phase);
+        const uint64_t b = vd + vs * TILE16;
+        wait(&p_full[i], tiles & 1);
+        tc::fence_after_sync();
+        if (leader) {
 #pragma unroll
-            for (int k = 0; k < PT_KEYS / 16; ++k)
-              tc::mma_f16_ta(tmem + 2 * PT_KEYS + i * D, tmem + i * PT_KEYS + k * 8,
-                             tc::sdesc_mn<S::BOXB>(b0 + k * 16 * S::BOXB, PT_KEYS * S::BOXB), id_o, (t > 0 || k > 0) ? 1u : 0u);
-            if (!more) tc::commit(&o_full[i]);
-            if (i == w.nsub - 1) tc::commit(&kv_empty[vs]);
-          }
-          if (more) {
-            if (i == 0) wait(&kv_full[ks], ((n + 2) / SLOTS) & 1);
-            scores(i, ks);
-            if (i == w.nsub - 1 && lane == 0) {
-              tc::commit(&kv_empty[ks]);
-              if (t + 2 == w.ntile) tc::commit(&q_empty);
-            }
-          }
-          __syncwarp();
+          for (int k = 0; k < PT_HEAD / 16; ++k) tc::mma_f16_ta(to, ts + k * 8, b + k * S::BOXB, id_o, (t > 0 || k > 0) ? 1u : 0u);
         }
+        wait(&p_tail[i], tiles & 1);
+        tc::fence_after_sync();
+        if (leader) {
+#pragma unroll
+          for (int k = PT_HEAD / 16; k < PT_KEYS / 16; ++k) tc::mma_f16_ta(to, ts + k * 8, b + k * S::BOXB, id_o, 1u);
+          if (!more) tc::commit(&o_full[i]);
+          if (more) scores();
+          tc::commit(&kv_empty[vs]);
+          if (more && t + 2 == ntile) tc::commit(&q_empty);
+        }
+        if (more) bump();
       }
     }
+   }
   } else {
     // ------------------------------------------------ softmax of row tile `sub`
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PT_REGS_SOFTMAX));
     const int sub = warp >> 2, r = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + lanes + sub * PT_KEYS, to = tmem + lanes + 2 * PT_KEYS + sub * D;
     const bool cap = p.q.softcap > 0.f;
     const float c = (cap ? 1.f : p.q.scaling) * 1.44269504f;              // scores are powers of two of s c
     const float cap_in = cap ? 2.f * 1.44269504f * p.q.scaling / p.q.softcap : 0.f;
-    uint32_t tiles = 0, items = 0;
-    for (; w.live(); w.next(p)) {
-      w.open(p, g.tps);
+    const int ti = r / p.grp, gi = r - ti * p.grp;
+    uint32_t tiles = 0, outs = 0, next = 0, before;   // before: tiles of the block's earlier segments
+    for (uint32_t items = 0;; ++items) {
+      if (ok && !mbar_wait_bounded(&q_full, items & 1)) ok = false;
+      const PtSeg w = seg[items & 1];
+      before = next;
+      next += w.ntile;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_empty);
+      if (!ok || w.ntile == 0) break;
       if (sub >= w.nsub) continue;
-      int i, head;
-      const bool have = paged_row(p, w.at.it, w.at.hp, w.at.rt, sub * rows + r, i, head) && r < rows;
-      const int place = p.q.causal ? w.at.it.base + i : 0x7fffffff;
+      const int tok = sub * g.tps + ti;
+      const bool have = ti < g.tps && gi < w.heads && tok < w.tok;
+      const int place = p.q.causal ? w.base + tok : 0x7fffffff;
       // key tiles inside [free_lo, free_hi] are seen by every row of this row tile
-      const int64_t t0 = (int64_t)w.at.rt * p.tpt + sub * g.tps;
-      const int64_t free_hi = p.q.causal ? min((int64_t)w.hi - 1, (int64_t)w.at.it.base + t0) : (int64_t)w.hi - 1;
-      const int64_t free_lo = max((int64_t)w.lo, p.q.window > 0 ? (int64_t)w.at.it.base + t0 + g.tps - p.q.window : (int64_t)0);
+      const int64_t t0 = (int64_t)w.base + sub * g.tps;
+      const int64_t free_hi = p.q.causal ? min((int64_t)w.hi - 1, t0) : (int64_t)w.hi - 1;
+      const int64_t free_lo = max((int64_t)w.lo, p.q.window > 0 ? t0 + g.tps - p.q.window : (int64_t)0);
       float m = -INFINITY, l = 0.f;
       for (int t = 0; t < w.ntile; ++t, ++tiles) {
         if (ok && !mbar_wait_bounded(&s_full[sub], tiles & 1)) ok = false;
         tc::fence_after_sync();
-        // The scores are read twice, 32 columns at a time (the second time as
-        // exponents): a row of 128 does not fit the registers next to the rest.
-        uint32_t buf[2][32];
+        uint32_t su[PT_KEYS];
+#pragma unroll
+        for (int x = 0; x < PT_KEYS; x += 32) tc::ld_32x32(ts + x, su + x);
+#pragma unroll
+        for (int x = 0; x < PT_KEYS; x += 32) tc::wait_ld32(su + x);
+        if (cap) {
+#pragma unroll
+          for (int x = 0; x < PT_KEYS; ++x)
+            su[x] = __float_as_uint(p.q.softcap * (1.f - __fdividef(2.f, 1.f + ex2(__uint_as_float(su[x]) * cap_in))));
+        }
         const int64_t j0 = w.j00 + (int64_t)t * PT_KEYS;
-        const bool masked = j0 < free_lo || j0 + PT_KEYS - 1 > free_hi;
-        // columns [bot, top] are seen
-        const int top = (int)min((int64_t)PT_KEYS, min((int64_t)w.hi - 1, (int64_t)place) - j0);
-        const int bot = (int)max((int64_t)0, max((int64_t)w.lo, p.q.window > 0 ? (int64_t)place - p.q.window + 1 : (int64_t)0) - j0);
-        float mx[4] = {m, m, m, m};
-        tc::ld_32x32(ts, buf[0]);
+        if (j0 < free_lo || j0 + PT_KEYS - 1 > free_hi) {
+          // columns [bot, top] are seen
+          const int top = (int)min((int64_t)PT_KEYS, min((int64_t)w.hi - 1, (int64_t)place) - j0);
+          const int bot = (int)max((int64_t)0, max((int64_t)w.lo, p.q.window > 0 ? (int64_t)place - p.q.window + 1 : (int64_t)0) - j0);
 #pragma unroll
-        for (int x = 0; x < PT_KEYS; x += 32) {
-          uint32_t *su = buf[(x / 32) & 1];
-          tc::wait_ld32(su);
-          if (x + 32 < PT_KEYS) tc::ld_32x32(ts + x + 32, buf[(x / 32 + 1) & 1]);
-          if (masked || cap) {                 // put the score itself back
-#pragma unroll
-            for (int y = 0; y < 32; ++y) {
-              float v = __uint_as_float(su[y]);
-              if (cap) v = p.q.softcap * (1.f - __fdividef(2.f, 1.f + ex2(v * cap_in)));
-              if (x + y > top || x + y < bot) v = -INFINITY;
-              su[y] = __float_as_uint(v);
+          for (int x = 0; x < PT_KEYS; ++x)
+            if (x > top || x < bot) su[x] = 0xff800000u;
+          if (j0 < w.lo || j0 + PT_KEYS > w.hi) {
+            // Dead rows of the V tile: each group clears them for its own
+            // product, which waits for p_full below.
+            const uint32_t n = 2 * (before + t) + 1, vs = n % SLOTS;
+            if (ok && !mbar_wait_bounded(&kv_full[vs], (n / SLOTS) & 1)) ok = false;
+            const int dl = (int)max((int64_t)0, w.lo - j0), dh = (int)max((int64_t)0, min((int64_t)PT_KEYS, w.hi - j0));
+            if (r < dl || r >= dh) {
+#pragma unroll 1
+              for (int y = 0; y < D / 8; ++y)
+                *reinterpret_cast<uint4 *>(ring + vs * S::TILE + (y / (S::BOX / 8)) * (PT_KEYS * S::BOXB) + r * S::BOXB +
+                                           (y % (S::BOX / 8)) * 16) = make_uint4(0, 0, 0, 0);
             }
-            tc::st_32x32(ts + x, su);
-          }
-#pragma unroll
-          for (int y = 0; y < 32; y += 8) {
-#pragma unroll
-            for (int z = 0; z < 4; ++z)
-              mx[z] = fmaxf(mx[z], fmaxf(__uint_as_float(su[y + 2 * z]), __uint_as_float(su[y + 2 * z + 1])));
+            tc::fence_proxy_async_smem();
           }
         }
-        if (masked || cap) tc::wait_st();
-        tc::ld_32x32(ts, buf[0]);
-        const float mn = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        float mx[8];
+#pragma unroll
+        for (int y = 0; y < 8; ++y) mx[y] = m;
+#pragma unroll
+        for (int x = 0; x < PT_KEYS; x += 16) {
+#pragma unroll
+          for (int y = 0; y < 8; ++y)
+            mx[y] = fmaxf(mx[y], fmaxf(__uint_as_float(su[x + 2 * y]), __uint_as_float(su[x + 2 * y + 1])));
+        }
+        const float mn = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])));
         if (t == 0) {
           m = mn;
         } else if (__any_sync(KIV_FULL_MASK, (mn - m) * c > PT_LAZY)) {   // (-inf) - (-inf) is NaN: no growth
@@ -406,13 +470,13 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
           l *= f;
           m = mn;
 #pragma unroll 1
-          for (int x = 0; x < D; x += 32) {
-            uint32_t o[32];
-            tc::ld_32x32(to + x, o);
-            tc::wait_ld32(o);
+          for (int x = 0; x < D; x += 16) {
+            uint32_t o[16];
+            tc::ld_32x16(to + x, o);
+            tc::wait_ld16(o);
 #pragma unroll
-            for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
-            tc::st_32x32(to + x, o);
+            for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
+            tc::st_32x16(to + x, o);
           }
         }
         const float2 c2 = make_float2(c, c);
@@ -421,35 +485,39 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
         for (int x = 0; x < PT_KEYS; x += 32) {
-          uint32_t *su = buf[(x / 32) & 1];
-          tc::wait_ld32(su);
-          if (x + 32 < PT_KEYS) tc::ld_32x32(ts + x + 32, buf[(x / 32 + 1) & 1]);
           uint32_t pk[16];
 #pragma unroll
           for (int y = 0; y < 32; y += 2) {
-            float2 e = __ffma2_rn(make_float2(__uint_as_float(su[y]), __uint_as_float(su[y + 1])), c2, n2);
+            float2 e = __ffma2_rn(make_float2(__uint_as_float(su[x + y]), __uint_as_float(su[x + y + 1])), c2, n2);
             e.x = ex2(e.x);
             e.y = ex2(e.y);
             sum[(y >> 1) & 1] = __fadd2_rn(sum[(y >> 1) & 1], e);
             pk[y / 2] = pt_pack<BF>(e.x, e.y);
           }
-          tc::st_32x16(ts + x / 2, pk);        // over columns that were read before
+          tc::st_32x16(ts + x / 2, pk);
+          if (x + 32 == PT_HEAD) {             // the product of these keys can begin
+            tc::wait_st();
+            tc::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[sub]);
+          }
         }
         l += (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y);
         tc::wait_st();
         tc::fence_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[sub]);
+        if (lane == 0) mbar_arrive(&p_tail[sub]);
       }
       // ---- the item's rows
-      if (ok && !mbar_wait_bounded(&o_full[sub], items & 1)) ok = false;
-      ++items;
+      if (ok && !mbar_wait_bounded(&o_full[sub], outs & 1)) ok = false;
+      ++outs;
       tc::fence_after_sync();
       const float mnat = m * c * 0.693147181f;
-      const bool whole = !w.sg.head && !w.sg.tail;
+      const bool whole = w.part < 0;
       const float inv = l > 0.f ? 1.f / l : 0.f;
-      T *dst = have && whole ? paged_out<T>(p, w.at.it, i, head) : nullptr;
-      float *part = paged_part(p, 2 * (int64_t)blockIdx.x + (w.sg.head ? 0 : 1), sub * rows + r);
+      const int head = w.head0 + gi;
+      T *dst = static_cast<T *>(p.q.out) + (w.q0 + tok) * p.q.out_stride_t + head * p.q.out_stride_h;
+      float *part = paged_part(p, w.part, sub * rows + r);
 #pragma unroll
       for (int x = 0; x < D; x += 32) {
         uint32_t o[32];
@@ -473,7 +541,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
       }
       if (have) {
         if (whole) {
-          paged_lse(p, w.at.it, i, head, mnat, l);
+          if (p.q.lse) p.q.lse[(w.q0 + tok) * p.q.num_query_heads + head] = l > 0.f ? mnat + logf(l) : -INFINITY;
         } else {
           part[D] = mnat;
           part[D + 1] = l;
