@@ -415,8 +415,10 @@ static int plan_calls(const kiv_paged *pc, const kiv_paged_query *q, PagedCall (
     PagedCall &t = c[n++];
     t.kernel = PAGED_TC;
     t.p = make_plan(pc, q, 128, 128);
-    t.p.tpt *= 2;
-    t.p.rows = 256;
+    if (D <= 128) {                 // two row tiles per item; at 256 TMEM holds the output of one
+      t.p.tpt *= 2;
+      t.p.rows = 256;
+    }
     if (!only_large) t.p.min_tokens = (int)((TC_ROWS - 1) / per) + 1;
     t.blocks = sm_count();
     size_call(t);

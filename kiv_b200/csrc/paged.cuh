@@ -124,7 +124,8 @@ bool paged_mma_head(int dtype, int D);
 int paged_mma_blocks(int D, int rows);
 kiv_status launch_paged_mma(const PagedPlan &p, int blocks, cudaStream_t s);
 
-// chunks, 16-bit rows, tcgen05 (paged_tc.cu); plan rows 256, kt 128, whole tokens per 128 rows
+// chunks, 16-bit rows, tcgen05 (paged_tc.cu, paged_tc256.cu); plan rows 256 (head_dim 256: 128), kt 128, whole
+// tokens per 128 rows
 bool paged_tc_eligible(const kiv_paged *pc, const kiv_paged_query *q);
 kiv_status launch_paged_tc(const PagedPlan &p, int blocks, cudaStream_t s);
 

@@ -29,22 +29,9 @@
 
 #include "internal.h"
 #include "paged.cuh"
-#include "tc.cuh"
+#include "paged_tc.cuh"
 
 namespace kiv {
-
-constexpr int PT_KEYS = 128;
-constexpr int PT_ROWS = 128;                   // of one row tile
-constexpr int PT_THREADS = 384;                // three warpgroups: two of softmax, one with the TMA and the MMA warp
-// registers per thread: 168 at launch, (2 x 208 + 88) x 128 = 168 x 384 after the split
-constexpr int PT_REGS_SOFTMAX = 208, PT_REGS_OTHER = 88;
-constexpr int PT_HEAD = 96;                    // keys of a tile whose P V product begins before the rest of P is there
-constexpr float PT_LAZY = 8.f;                 // growth (log2) that a row's reference may lag behind
-
-struct PagedTcGeom {
-  int tps;       // tokens per row tile
-  int br;        // rows per TMA box of a page: a power of two dividing page_size, at most 128
-};
 
 template <int D>
 struct TcShape {
@@ -54,119 +41,6 @@ struct TcShape {
   static constexpr int TILE = PT_KEYS * D * 2;           // bytes of a K, V or Q tile
   static constexpr int SLOTS = (232448 - 2048 - 2 * TILE) / TILE < 8 ? (232448 - 2048 - 2 * TILE) / TILE : 8;
   static constexpr size_t SMEM = 1024 + 2 * TILE + (size_t)SLOTS * TILE;
-};
-
-namespace tc {
-// A [TMEM, 16-bit pairs per column] x B [smem]
-__device__ __forceinline__ void mma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-// MN-major operand (rows = K index, contiguous along N) of a swizzled tile:
-// column blocks `block` bytes apart, 8-row groups 8 * row bytes apart
-template <int ROWB>
-__device__ __forceinline__ uint64_t sdesc_mn(uint32_t addr, uint32_t block) {
-  uint64_t d = 0;
-  d |= (uint64_t)((addr & 0x3FFFF) >> 4);
-  d |= (uint64_t)(block >> 4) << 16;
-  d |= (uint64_t)((8 * ROWB) >> 4) << 32;
-  d |= (uint64_t)1 << 46;
-  d |= (uint64_t)(ROWB == 128 ? 2 : 4) << 61;
-  return d;
-}
-__device__ __forceinline__ void ld_32x32(uint32_t taddr, uint32_t *r) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,"
-      "%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
-        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
-        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr)
-      : "memory");
-}
-__device__ __forceinline__ void st_32x32(uint32_t taddr, const uint32_t *r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
-      "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
-      "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]),
-      "r"(r[31])
-      : "memory");
-}
-__device__ __forceinline__ void st_32x16(uint32_t taddr, const uint32_t *r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
-}
-// completion of the loads into r: the registers are operands, so no use of
-// them can move before it
-__device__ __forceinline__ void wait_ld32(uint32_t *r) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
-                 "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),
-                 "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
-                 "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
-               :
-               : "memory");
-}
-__device__ __forceinline__ void wait_ld16(uint32_t *r) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
-               :
-               : "memory");
-}
-__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, int32_t x, int32_t y, int32_t z, uint64_t *bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
-          smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
-      : "memory");
-}
-}  // namespace tc
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// one lane of the (converged) warp
-__device__ __forceinline__ bool elect_one() {
-  uint32_t p;
-  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
-  return p != 0;
-}
-
-template <bool BF>
-__device__ __forceinline__ uint32_t pt_pack(float x, float y) {
-  if constexpr (BF) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-    return *reinterpret_cast<const uint32_t *>(&h);
-  } else {
-    const __half2 h = __floats2half2_rn(x, y);
-    return *reinterpret_cast<const uint32_t *>(&h);
-  }
-}
-
-// One segment of the block's stretch, as the TMA warp tells the others.
-struct PtSeg {
-  int ntile;       // 0: no more
-  int nsub;        // row tiles that have tokens
-  int lo, hi;      // live keys
-  int64_t j00;     // first key of its first key tile
-  int64_t q0;      // packed row of token 0 of the item's first row tile
-  int tok;         // tokens from there on
-  int base;        // place of that token (causal), or the length
-  int head0, heads;   // its query heads
-  int part;        // workspace slot, or -1: the rows are finished here
 };
 
 template <bool BF, int D>
@@ -227,28 +101,12 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
    if (warp == 8) {
     // ------------------------------------------------ TMA
     uint32_t n = 0, items = 0;
-    const int per = p.q.num_query_heads / p.pc.num_kv_heads;
     for (;; ++items) {
       const bool live = at.it.s.b >= 0 && at.unit < at.end;
       PtSeg sg = {};
       PagedSegment cut = {};
       int kvh = 0;
-      if (live) {
-        cut = paged_segment(p, at);
-        paged_range(p, at.it, at.rt, sg.lo, sg.hi);
-        sg.hi = min(sg.hi, at.it.s.len);
-        sg.j00 = ((int64_t)sg.lo / PT_KEYS + cut.t0) * PT_KEYS;
-        sg.ntile = cut.t1 - cut.t0;
-        const int first = at.rt * p.tpt;
-        sg.q0 = at.it.s.q0 + first;
-        sg.tok = min(at.it.s.n - first, p.tpt);
-        sg.nsub = sg.tok > g.tps ? 2 : 1;
-        sg.base = p.q.causal ? at.it.base + first : at.it.s.len;
-        kvh = at.hp / p.hs;
-        sg.head0 = kvh * per + (at.hp % p.hs) * p.grp;
-        sg.heads = min(p.grp, per - (at.hp % p.hs) * p.grp);
-        sg.part = cut.head ? 2 * (int)blockIdx.x : cut.tail ? 2 * (int)blockIdx.x + 1 : -1;
-      }
+      if (live) sg = pt_segment(p, at, g.tps, cut, kvh);
       if (items > 0 && ok && !mbar_wait_bounded(&q_empty, (items - 1) & 1)) ok = false;
       if (lane == 0) {
         seg[items & 1] = sg;
@@ -270,18 +128,9 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
       const int nbox = PT_KEYS / g.br;
       const int32_t *table = p.pc.block_table + at.it.s.b * p.pc.table_stride;
       auto lookup = [&](int t, int32_t &page, int32_t &row) {
-        page = -1;                             // outside: the box reads as zeros
+        page = -1;
         row = 0;
-        const int64_t j = sg.j00 + (int64_t)t * PT_KEYS + lane * g.br;
-        if (t < sg.ntile && lane < nbox && j < sg.hi && j + g.br > sg.lo) {
-          const uint32_t pg = (uint32_t)j / (uint32_t)p.pc.page_size;
-          row = (int32_t)((uint32_t)j - pg * (uint32_t)p.pc.page_size);
-          page = table[pg];
-          if (page < 0 || page >= p.pc.num_pages) {
-            paged_error(p.pc.errors, KIV_ERRBIT_BLOCK_TABLE);
-            page = -1;
-          }
-        }
+        if (t < sg.ntile && lane < nbox) pt_lookup(p, table, sg, sg.j00 + (int64_t)t * PT_KEYS + lane * g.br, g.br, page, row);
       };
       int32_t page, row;
       lookup(0, page, row);
@@ -560,13 +409,36 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
 // ------------------------------------------------------------------ host
 bool paged_tc_eligible(const kiv_paged *pc, const kiv_paged_query *q) {
   const int D = pc->head_dim, per = q->num_query_heads / pc->num_kv_heads;
-  if (pc->dtype == KIV_DTYPE_F32 || !(D == 64 || D == 96 || D == 128) || pc->page_size % 8 != 0 || per > PT_ROWS) return false;
+  if (pc->dtype == KIV_DTYPE_F32 || !(D == 64 || D == 96 || D == 128 || D == 256) || pc->page_size % 8 != 0 || per > PT_ROWS) return false;
   if (!(q->scaling > 0.f) || pc->num_pages < 1) return false;   // the row maximum is taken before the scale
   // a dimension that is stepped needs a stride (an expanded one has 0)
   const bool k = (pc->num_pages == 1 || pc->k_stride_p > 0) && (pc->num_kv_heads == 1 || pc->k_stride_h > 0) && pc->k_stride_t > 0;
   const bool v = (pc->num_pages == 1 || pc->v_stride_p > 0) && (pc->num_kv_heads == 1 || pc->v_stride_h > 0) && pc->v_stride_t > 0;
   const bool qs = (pc->num_tokens == 1 || q->stride_t > 0) && (q->num_query_heads == 1 || q->stride_h > 0);
   return k && v && qs && getenv("KIV_DISABLE_TCGEN05") == nullptr;
+}
+
+// Tensor maps of the queries (box: `box` elements x the heads of a part x tps
+// tokens) and of the pages (`box` elements x br rows of one head and page).
+kiv_status pt_maps(const PagedPlan &p, int box, int br, int tps, CUtensorMapSwizzle sw, CUtensorMap *qm, CUtensorMap *km, CUtensorMap *vm) {
+  const int D = p.pc.head_dim;
+  auto stride = [D](int64_t size, int64_t st) { return (uint64_t)(size == 1 && st <= 0 ? D : st) * 2; };
+  {
+    const uint64_t dims[3] = {(uint64_t)D, (uint64_t)p.q.num_query_heads, (uint64_t)p.pc.num_tokens};
+    const uint64_t st[2] = {stride(p.q.num_query_heads, p.q.stride_h), stride(p.pc.num_tokens, p.q.stride_t)};
+    const uint32_t b[3] = {(uint32_t)box, (uint32_t)p.grp, (uint32_t)tps};
+    KIV_CHECK(encode_tiled(qm, p.pc.dtype, 3, p.q.q, dims, st, b, sw));
+  }
+  const uint64_t dims[4] = {(uint64_t)D, (uint64_t)p.pc.page_size, (uint64_t)p.pc.num_kv_heads, (uint64_t)p.pc.num_pages};
+  const uint32_t b[4] = {(uint32_t)box, (uint32_t)br, 1, 1};
+  {
+    const uint64_t st[3] = {stride(p.pc.page_size, p.pc.k_stride_t), stride(p.pc.num_kv_heads, p.pc.k_stride_h),
+                            stride(p.pc.num_pages, p.pc.k_stride_p)};
+    KIV_CHECK(encode_tiled(km, p.pc.dtype, 4, p.pc.k, dims, st, b, sw));
+  }
+  const uint64_t st[3] = {stride(p.pc.page_size, p.pc.v_stride_t), stride(p.pc.num_kv_heads, p.pc.v_stride_h),
+                          stride(p.pc.num_pages, p.pc.v_stride_p)};
+  return encode_tiled(vm, p.pc.dtype, 4, p.pc.v, dims, st, b, sw);
 }
 
 template <bool BF, int D>
@@ -576,27 +448,8 @@ static kiv_status launch_tc(const PagedPlan &p, int blocks, cudaStream_t s) {
   g.tps = PT_ROWS / p.grp;
   g.br = 8;
   while (g.br < PT_KEYS && p.pc.page_size % (2 * g.br) == 0) g.br *= 2;
-  const CUtensorMapSwizzle sw = S::BOX == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
   CUtensorMap qm, km, vm;
-  auto stride = [](int64_t size, int64_t st) { return (uint64_t)(size == 1 && st <= 0 ? D : st) * 2; };
-  {
-    const uint64_t dims[3] = {(uint64_t)D, (uint64_t)p.q.num_query_heads, (uint64_t)p.pc.num_tokens};
-    const uint64_t st[2] = {stride(p.q.num_query_heads, p.q.stride_h), stride(p.pc.num_tokens, p.q.stride_t)};
-    const uint32_t box[3] = {S::BOX, (uint32_t)p.grp, (uint32_t)g.tps};
-    KIV_CHECK(encode_tiled(&qm, p.pc.dtype, 3, p.q.q, dims, st, box, sw));
-  }
-  const uint64_t dims[4] = {(uint64_t)D, (uint64_t)p.pc.page_size, (uint64_t)p.pc.num_kv_heads, (uint64_t)p.pc.num_pages};
-  const uint32_t box[4] = {S::BOX, (uint32_t)g.br, 1, 1};
-  {
-    const uint64_t st[3] = {stride(p.pc.page_size, p.pc.k_stride_t), stride(p.pc.num_kv_heads, p.pc.k_stride_h),
-                            stride(p.pc.num_pages, p.pc.k_stride_p)};
-    KIV_CHECK(encode_tiled(&km, p.pc.dtype, 4, p.pc.k, dims, st, box, sw));
-  }
-  {
-    const uint64_t st[3] = {stride(p.pc.page_size, p.pc.v_stride_t), stride(p.pc.num_kv_heads, p.pc.v_stride_h),
-                            stride(p.pc.num_pages, p.pc.v_stride_p)};
-    KIV_CHECK(encode_tiled(&vm, p.pc.dtype, 4, p.pc.v, dims, st, box, sw));
-  }
+  KIV_CHECK(pt_maps(p, S::BOX, g.br, g.tps, S::BOX == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, &qm, &km, &vm));
   cudaFuncSetAttribute(paged_tc_kernel<BF, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM);
   KIV_CHECK(cuda_status(launch_pdl(paged_tc_kernel<BF, D>, dim3((unsigned)blocks), dim3(PT_THREADS), S::SMEM, s, 1, qm, km, vm, p, g),
                         "paged_attend (chunk)"));
@@ -608,6 +461,7 @@ kiv_status launch_paged_tc(const PagedPlan &p, int blocks, cudaStream_t s) {
   switch (p.pc.head_dim) {
     case 64: return bf ? launch_tc<true, 64>(p, blocks, s) : launch_tc<false, 64>(p, blocks, s);
     case 96: return bf ? launch_tc<true, 96>(p, blocks, s) : launch_tc<false, 96>(p, blocks, s);
+    case 256: return launch_paged_tc256(p, blocks, s);
     default: return bf ? launch_tc<true, 128>(p, blocks, s) : launch_tc<false, 128>(p, blocks, s);
   }
 }
