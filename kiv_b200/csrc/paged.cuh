@@ -41,22 +41,15 @@ __device__ __forceinline__ PagedSeq paged_seq(const kiv_paged &pc, int b) {
   return s;
 }
 
-// The sequence of packed row `tok` (b = -1: none), found by the whole block in
-// one round trip: how many sequences end at or before the row.
-__device__ __forceinline__ PagedSeq paged_find_seq(const kiv_paged &pc, int64_t tok) {
+// The first sequence that ends behind packed row `tok`, found by the whole
+// block in one round trip: how many end at or before it.
+__device__ __forceinline__ int paged_find_seq(const kiv_paged &pc, int64_t tok) {
   int before = 0;
   for (int b0 = 0; b0 < pc.batch; b0 += blockDim.x) {
     const int b = b0 + threadIdx.x;
     before += __syncthreads_count(b < pc.batch && (int64_t)pc.q_starts[b + 1] <= tok);
   }
-  PagedSeq s;
-  s.b = -1;
-  if (before >= pc.batch) return s;
-  s.q0 = pc.q_starts[before];
-  s.n = pc.q_starts[before + 1] - pc.q_starts[before];
-  s.len = pc.seq_lens[before];
-  if (s.q0 <= tok) s.b = before;
-  return s;
+  return before;
 }
 
 // ---------------------------------------------------------------------------
