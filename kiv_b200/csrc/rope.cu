@@ -9,12 +9,11 @@
 // sin rows, weights) is shared by the heads of a token.  A group of GL lanes
 // takes one token and `hc` of its heads: it asks for its first rows, then loads
 // the token's cos and sin and its weight elements into registers -- 16 bytes at
-// a time where they line up -- and walks the heads, a 16-byte vector per lane
-// and row (two for rows of more than 512 bytes), UN rows in flight.  The
-// partner of a half-split pair sits rot_dim / 2 elements away, i.e. in another
-// lane of the group: one shuffle, with no shared memory.  (A block per token,
-// rows asked for after cos and sin, ran at 1.7 TB/s: three dependent round
-// trips for one row per thread.)
+// a time where they line up -- and walks the heads, RP_UN rows in flight.  A
+// lane holds two 16-byte vectors of a row, and for half-split pairs these are
+// the two sides of the same pairs: no exchange between lanes, and one cos and
+// sin per pair.  (One vector per lane, the other side by shuffles, took four
+// times the instructions and 53 us where this takes RP_TIME.)
 #include <algorithm>
 
 #include "internal.h"
@@ -23,6 +22,7 @@
 namespace kiv {
 
 constexpr int RP_THREADS = 256;
+constexpr int RP_UN = 4;         // rows in flight: 512 threads x 4 x 32 B = 64 KB per SM
 
 struct TurnArgs {
   kiv_turn t;
@@ -31,9 +31,9 @@ struct TurnArgs {
   int rows[2];             // heads of each
   int tokens;              // per batch row (rope) / packed (append)
   int head_dim;
-  int64_t ntok;            // all of them
-  int hc, nch;             // heads per group; groups per token
-  int vec_cs, vec_w;       // cos / sin rows, weights can be read 16 (interleaved: 8 or 16) bytes at a time
+  uint32_t ntok;           // all of them
+  int hc;                  // heads per group
+  int vec_cs, vec_w;       // cos / sin rows, weights can be read 16 bytes at a time
   int64_t *errors;
   kiv_paged pc;            // append only
 };
@@ -48,167 +48,160 @@ __device__ __forceinline__ int64_t ld_pos(const kiv_turn &t, int axis, int64_t b
   return t.pos_is_i64 ? static_cast<const int64_t *>(t.positions)[o] : (int64_t)static_cast<const int32_t *>(t.positions)[o];
 }
 
-// N consecutive values at p[i ..), read as vectors (16-bit: T)
+// N consecutive values at p[i ..), read as vectors (N values fill a 16-byte row vector)
 template <typename T, int N>
 __device__ __forceinline__ void ld_vec(const void *p, int64_t i, bool f32, float *out) {
   if (f32) {
     const float *q = static_cast<const float *>(p) + i;
 #pragma unroll
-    for (int e = 0; e < N; e += (N % 4 == 0 ? 4 : 2)) {
-      if constexpr (N % 4 == 0) {
-        const float4 v = *reinterpret_cast<const float4 *>(q + e);
-        out[e] = v.x;
-        out[e + 1] = v.y;
-        out[e + 2] = v.z;
-        out[e + 3] = v.w;
-      } else {
-        const float2 v = *reinterpret_cast<const float2 *>(q + e);
-        out[e] = v.x;
-        out[e + 1] = v.y;
-      }
+    for (int e = 0; e < N; e += 4) {
+      const float4 v = *reinterpret_cast<const float4 *>(q + e);
+      out[e] = v.x;
+      out[e + 1] = v.y;
+      out[e + 2] = v.z;
+      out[e + 3] = v.w;
     }
   } else if constexpr (sizeof(T) == 2) {
-    const T *q = static_cast<const T *>(p) + i;
-    if constexpr (N == 8) {
-      Elem<T>::unpack(ld16(q), out);
-    } else {
-      static_assert(N == 4, "8 or 4 values");
-      const uint2 v = *reinterpret_cast<const uint2 *>(q);
-      float f[8];
-      Elem<T>::unpack(make_uint4(v.x, v.y, 0, 0), f);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) out[e] = f[e];
-    }
+    Elem<T>::unpack(ld16(static_cast<const T *>(p) + i), out);
   }
 }
 
-// GL lanes per row, VPL vectors per lane.  APPEND: in/out 0 are keys (turned),
+// GL lanes per row, two vectors per lane.  APPEND: in/out 0 are keys (turned),
 // 1 are values (copied), and the destination row comes from the block table.
-template <typename T, int GL, int VPL, bool APPEND>
-__global__ void __launch_bounds__(RP_THREADS) turn_kernel(const __grid_constant__ TurnArgs a) {
+template <typename T, int GL, bool APPEND, bool NORM>
+__global__ void __launch_bounds__(RP_THREADS, !NORM && sizeof(T) == 4 ? 3 : 2) turn_kernel(const __grid_constant__ TurnArgs a) {
   constexpr int V = Elem<T>::V;
   constexpr int GROUPS = RP_THREADS / GL;
-  constexpr int UN = VPL == 1 ? 4 : 2;
   // rows of pairs that do not line up with the vectors trade partners here
-  __shared__ float s_row[GROUPS][GL * VPL * V];
+  __shared__ float s_row[GROUPS][GL * 2 * V];
   const int D = a.head_dim, nv = D / V;
   const int lane = threadIdx.x % GL, grp = threadIdx.x / GL;
   const unsigned gmask = GL == 32 ? KIV_FULL_MASK : ((1u << GL) - 1) << ((threadIdx.x & 31) / GL * GL);
   griddep_wait();
-  const int64_t gid = (int64_t)blockIdx.x * GROUPS + grp, tok = gid / a.nch;
-  const int ch = (int)(gid - tok * a.nch);
   const kiv_turn &t = a.t;
+  const uint32_t tok = blockIdx.x * GROUPS + grp;
+  const int r_first = blockIdx.y * a.hc, r_end = min(a.rows[0] + a.rows[1], r_first + a.hc);
   bool live = tok < a.ntok;
-  const int total = a.rows[0] + a.rows[1], r_end = min(total, (ch + 1) * a.hc);
-  const int64_t b = APPEND || !live ? 0 : tok / a.tokens, i = live ? tok - b * a.tokens : 0;
+  const uint32_t b = APPEND || !live ? 0 : tok / (uint32_t)a.tokens, i = live ? tok - b * (uint32_t)a.tokens : 0;
 
-  auto source = [&](int r) {
-    const int which = r < a.rows[0] ? 0 : 1;
-    const kiv_rows &in = a.in[which];
-    return static_cast<const T *>(in.p) + b * in.stride_b + (r - (which ? a.rows[0] : 0)) * in.stride_h + i * in.stride_t;
-  };
-  uint4 raw[UN][VPL];
+  // ---- this lane's vectors: the sides of a pair (half-split), else neighbours
+  const int half = t.rot_dim / 2;
+  const bool rotate = a.turned && t.cos != nullptr;
+  const bool lined = t.interleaved ? t.rot_dim % V == 0 : half % V == 0;   // pairs line up with the vectors
+  const int hv = rotate && lined && !t.interleaved ? half / V : 0;
+  const int va = lane < hv ? lane : 2 * hv + 2 * (lane - hv), vb = lane < hv ? lane + hv : va + 1;
+  const bool has_a = live && va < nv, has_b = live && vb < nv;
+
+  const T *src[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) src[k] = static_cast<const T *>(a.in[k].p) + b * a.in[k].stride_b + i * a.in[k].stride_t;
+  uint4 ra[RP_UN], rb[RP_UN];
   auto fetch = [&](int r0) {
 #pragma unroll
-    for (int u = 0; u < UN; ++u) {
-#pragma unroll
-      for (int j = 0; j < VPL; ++j) {
-        const int vi = lane + j * GL;
-        raw[u][j] = make_uint4(0, 0, 0, 0);
-        if (live && r0 + u < r_end && vi < nv) raw[u][j] = ld16(source(r0 + u) + vi * V);
+    for (int u = 0; u < RP_UN; ++u) {
+      const int r = r0 + u;
+      const T *row = r < a.rows[0] ? src[0] + r * a.in[0].stride_h : src[1] + (r - a.rows[0]) * a.in[1].stride_h;
+      ra[u] = rb[u] = make_uint4(0, 0, 0, 0);
+      if (r < r_end) {
+        if (has_a) ra[u] = ld16(row + va * V);
+        if (has_b) rb[u] = ld16(row + vb * V);
       }
     }
   };
-  fetch(ch * a.hc);
+  fetch(r_first);
 
   // ---- where the token belongs
-  int64_t place = tok, koff = 0, voff = 0;
+  T *dst[2];
+  int64_t place = tok;
   if (APPEND) {
-    int sb = paged_find_seq(a.pc, (int64_t)blockIdx.x * GROUPS / a.nch);   // of the block's first token
-    while (live && sb < a.pc.batch && (int64_t)a.pc.q_starts[sb + 1] <= tok) ++sb;
-    const bool mine = live && sb < a.pc.batch && (int64_t)a.pc.q_starts[sb] <= tok;   // else: in no sequence
-    live = mine;
-    if (mine) {
+    int sb = paged_find_seq(a.pc, (int64_t)blockIdx.x * GROUPS);   // of the block's first token
+    while (live && sb < a.pc.batch && (int64_t)a.pc.q_starts[sb + 1] <= (int64_t)tok) ++sb;
+    live = live && sb < a.pc.batch && (int64_t)a.pc.q_starts[sb] <= (int64_t)tok;   // else: in no sequence
+    if (live) {
       place = (int64_t)a.pc.seq_lens[sb] - a.pc.q_starts[sb + 1] + tok;
       live = place >= 0 && place < a.pc.table_width * a.pc.page_size;
       if (!live && lane == 0) paged_error(a.errors, KIV_ERRBIT_SEQ_LEN);
     }
+    dst[0] = dst[1] = nullptr;
     if (live) {
-      const int32_t page = a.pc.block_table[sb * a.pc.table_stride + place / a.pc.page_size];
-      const int64_t r = place % a.pc.page_size;
+      const uint32_t pi = (uint32_t)place / (uint32_t)a.pc.page_size;
+      const int64_t r = (uint32_t)place - pi * (uint32_t)a.pc.page_size;
+      const int32_t page = a.pc.block_table[sb * a.pc.table_stride + pi];
       if (page < 0 || page >= a.pc.num_pages) {
         live = false;
         if (lane == 0) paged_error(a.errors, KIV_ERRBIT_BLOCK_TABLE);
       } else {
-        koff = page * a.pc.k_stride_p + r * a.pc.k_stride_t;
-        voff = page * a.pc.v_stride_p + r * a.pc.v_stride_t;
+        dst[0] = static_cast<T *>(a.pc.k) + page * a.pc.k_stride_p + r * a.pc.k_stride_t;
+        dst[1] = static_cast<T *>(a.pc.v) + page * a.pc.v_stride_p + r * a.pc.v_stride_t;
       }
     }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) dst[k] = static_cast<T *>(a.out[k].p) + b * a.out[k].stride_b + i * a.out[k].stride_t;
   }
 
-  // ---- cos, sin (sign of the pair's side folded in) of this lane's elements
-  const int half = t.rot_dim / 2;
-  const bool rotate = a.turned && t.cos != nullptr;
-  const bool lined = t.interleaved ? t.rot_dim % V == 0 : half % V == 0;   // pairs line up with the vectors
-  float c[VPL][V], s[VPL][V];
-#pragma unroll
-  for (int j = 0; j < VPL; ++j)
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      c[j][e] = 1.f;
-      s[j][e] = 0.f;
-    }
-  bool poison = false;
+  // ---- cos, sin of this lane's pairs: pair e of (a, b), or, interleaved, pairs
+  // e < V / 2 of a and the others of b
+  float c[V], s[V];
+  bool poison = false, turns = false;          // turns: this lane has pairs
+  auto pair_of = [&](int e) { return t.interleaved ? (e < V / 2 ? va * (V / 2) + e : vb * (V / 2) + e - V / 2) : va * V + e; };
+  auto row_of = [&](int pair, int64_t row0) -> int64_t {   // of the tables, -1: none
+    if (!t.pair_axes) return row0;
+    const int ax = t.pair_axes[pair];
+    if (ax < 0 || ax >= t.axes) return -1;
+    return t.positions ? ld_pos(t, ax, b, i) : place;
+  };
+  int64_t row0 = place;
+  int ax[V];
   if (rotate) {
     const bool f32 = t.cs_dtype == KIV_DTYPE_F32;
     bool bad = false;
     if (live) {
-      const int64_t row0 = t.positions ? (t.pair_axes ? 0 : ld_pos(t, 0, b, i)) : place;
+      if (t.positions) row0 = t.pair_axes ? 0 : ld_pos(t, 0, b, i);
       bad = row0 < 0 || row0 >= t.cs_rows;
+      if (lined) {
+        turns = t.interleaved ? va * V < t.rot_dim : lane < hv;
+        const bool both = !t.interleaved || vb * V < t.rot_dim;      // interleaved: b may lie behind the pairs
+        bool same = true;                                            // this lane's pairs turn by one row
+        if (turns && t.pair_axes) {
+          // the axes' positions and the pairs' axes in one round trip
+          int64_t at[4];
 #pragma unroll
-      for (int j = 0; j < VPL; ++j) {
-        const int x0 = (lane + j * GL) * V;
-        if (bad || x0 >= t.rot_dim) continue;
-        if (a.vec_cs && lined && !t.pair_axes) {
-          if (t.interleaved) {
-            float cc[V / 2], ss[V / 2];
-            ld_vec<T, V / 2>(t.cos, row0 * t.cs_stride + x0 / 2, f32, cc);
-            ld_vec<T, V / 2>(t.sin, row0 * t.cs_stride + x0 / 2, f32, ss);
+          for (int k = 0; k < 4; ++k) at[k] = t.positions ? (k < t.axes ? ld_pos(t, k, b, i) : -1) : place;
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-              c[j][e] = cc[e / 2];
-              s[j][e] = e & 1 ? ss[e / 2] : -ss[e / 2];
-            }
-          } else {
-            const bool second = x0 >= half;
-            ld_vec<T, V>(t.cos, row0 * t.cs_stride + (second ? x0 - half : x0), f32, c[j]);
-            ld_vec<T, V>(t.sin, row0 * t.cs_stride + (second ? x0 - half : x0), f32, s[j]);
-            if (!second) {
+          for (int e = 0; e < V; ++e) ax[e] = both || e < V / 2 ? t.pair_axes[pair_of(e)] : -1;
 #pragma unroll
-              for (int e = 0; e < V; ++e) s[j][e] = -s[j][e];
-            }
+          for (int e = 1; e < V; ++e) same = same && ax[e] == ax[0];
+          if (same) {
+            const int k = ax[0];
+            row0 = k < 0 || k >= t.axes ? -1 : !t.positions ? place : k == 0 ? at[0] : k == 1 ? at[1] : k == 2 ? at[2] : k == 3 ? at[3] : ld_pos(t, k, b, i);
+            bad = row0 < 0 || row0 >= t.cs_rows;
           }
-        } else {
+        }
+        if (turns && !bad && a.vec_cs && same && both) {
+          ld_vec<T, V>(t.cos, row0 * t.cs_stride + pair_of(0), f32, c);
+          ld_vec<T, V>(t.sin, row0 * t.cs_stride + pair_of(0), f32, s);
+        } else if (turns && !bad) {
 #pragma unroll
           for (int e = 0; e < V; ++e) {
-            const int x = x0 + e;
-            if (x >= t.rot_dim) continue;
-            const int pair = t.interleaved ? x >> 1 : (x < half ? x : x - half);
-            const bool second = t.interleaved ? (x & 1) != 0 : x >= half;
-            int64_t row = row0;
-            if (t.pair_axes) {
-              const int ax = t.pair_axes[pair];
-              const bool okay = ax >= 0 && ax < t.axes;
-              row = !okay ? -1 : t.positions ? ld_pos(t, ax, b, i) : place;
-            }
-            if (row < 0 || row >= t.cs_rows) {
-              bad = true;
-            } else {
-              c[j][e] = ld_as_float<T>(t.cos, row * t.cs_stride + pair, f32);
-              const float sn = ld_as_float<T>(t.sin, row * t.cs_stride + pair, f32);
-              s[j][e] = second ? sn : -sn;
+            c[e] = 1.f;
+            s[e] = 0.f;
+            if (both || e < V / 2) {
+              const int pair = pair_of(e);
+              const int64_t row = row_of(pair, row0);
+              if (row < 0 || row >= t.cs_rows) {
+                bad = true;
+              } else {
+                c[e] = ld_as_float<T>(t.cos, row * t.cs_stride + pair, f32);
+                s[e] = ld_as_float<T>(t.sin, row * t.cs_stride + pair, f32);
+              }
             }
           }
+        }
+      } else if (!bad && t.pair_axes) {
+        for (int pair = lane; pair < half; pair += GL) {
+          const int64_t row = row_of(pair, row0);
+          bad = bad || row < 0 || row >= t.cs_rows;
         }
       }
     }
@@ -220,116 +213,100 @@ __global__ void __launch_bounds__(RP_THREADS) turn_kernel(const __grid_constant_
     }
   }
 
-  float w[VPL][V];
+  float w[NORM ? 2 * V : 1];
   int w_of = -1;   // whose weight is in the registers
-  for (int r0 = ch * a.hc; r0 < (ch + 1) * a.hc; r0 += UN) {      // the same count in every group
-    if (r0 > ch * a.hc) fetch(r0);
+  for (int r0 = r_first; r0 < r_first + a.hc; r0 += RP_UN) {       // the same count in every group
+    if (r0 > r_first) fetch(r0);
 #pragma unroll
-    for (int u = 0; u < UN; ++u) {
+    for (int u = 0; u < RP_UN; ++u) {
+      if (r0 - r_first + u >= a.hc) break;     // the same in every group
       const int r = r0 + u, which = r < a.rows[0] ? 0 : 1;
-      if (r0 - ch * a.hc + u >= a.hc) break;       // the same in every group
-      float x[VPL][V];
-#pragma unroll
-      for (int j = 0; j < VPL; ++j) Elem<T>::unpack(raw[u][j], x[j]);
       const bool turn = a.turned && !(APPEND && which == 1);
-      if (a.turned && t.norm) {   // the same for the whole block: the shuffles below are the whole warp's
+      float x[2 * V];
+      Elem<T>::unpack(ra[u], x);
+      Elem<T>::unpack(rb[u], x + V);
+      if constexpr (NORM) {
         const void *wp = which == 0 && !APPEND ? t.q_weight : t.k_weight;
         if (w_of != which) {
           w_of = which;
           const bool f32 = t.weight_dtype == KIV_DTYPE_F32;
 #pragma unroll
-          for (int j = 0; j < VPL; ++j) {
-            const int x0 = (lane + j * GL) * V;
+          for (int k = 0; k < 2; ++k) {
+            const int x0 = (k ? vb : va) * V;
             if (wp && a.vec_w && x0 < D) {
-              ld_vec<T, V>(wp, x0, f32, w[j]);
+              ld_vec<T, V>(wp, x0, f32, w + k * V);
 #pragma unroll
-              for (int e = 0; e < V; ++e) w[j][e] += t.weight_offset;
+              for (int e = 0; e < V; ++e) w[k * V + e] += t.weight_offset;
             } else {
 #pragma unroll
-              for (int e = 0; e < V; ++e) w[j][e] = wp && x0 + e < D ? t.weight_offset + ld_as_float<T>(wp, x0 + e, f32) : 1.f;
+              for (int e = 0; e < V; ++e) w[k * V + e] = wp && x0 + e < D ? t.weight_offset + ld_as_float<T>(wp, x0 + e, f32) : 1.f;
             }
           }
         }
         float ss = 0.f;
 #pragma unroll
-        for (int j = 0; j < VPL; ++j)
-#pragma unroll
-          for (int e = 0; e < V; ++e) ss = fmaf(x[j][e], x[j][e], ss);
+        for (int e = 0; e < 2 * V; ++e) ss = fmaf(x[e], x[e], ss);
 #pragma unroll
         for (int o = GL / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(KIV_FULL_MASK, ss, o);
         const float rs = rsqrtf(ss / (float)D + t.eps);
 #pragma unroll
-        for (int j = 0; j < VPL; ++j)
-#pragma unroll
-          for (int e = 0; e < V; ++e) x[j][e] = x[j][e] * rs * w[j][e];
+        for (int e = 0; e < 2 * V; ++e) x[e] = x[e] * rs * w[e];
       }
-      if (rotate) {
-        float p[VPL][V];
+      if (rotate && !lined) {
+        // any pair of any row of the tables: through shared memory, an element at a time
+        __syncwarp();
+#pragma unroll
+        for (int e = 0; e < 2 * V; ++e) s_row[grp][((e < V ? va : vb) * V + e % V) % (GL * 2 * V)] = x[e];
+        __syncwarp();
+        if (turn && live && !poison) {
+          const bool f32 = t.cs_dtype == KIV_DTYPE_F32;
+#pragma unroll 1
+          for (int e = 0; e < 2 * V; ++e) {
+            const int xi = (e < V ? va : vb) * V + e % V;
+            if (xi >= t.rot_dim) continue;
+            const int pair = t.interleaved ? xi >> 1 : (xi < half ? xi : xi - half);
+            const bool second = t.interleaved ? (xi & 1) != 0 : xi >= half;
+            const int64_t row = row_of(pair, row0);
+            const float cc = ld_as_float<T>(t.cos, row * t.cs_stride + pair, f32);
+            const float sn = ld_as_float<T>(t.sin, row * t.cs_stride + pair, f32);
+            const float me = s_row[grp][xi], other = s_row[grp][t.interleaved ? xi ^ 1 : (second ? xi - half : xi + half)];
+            const float y = fmaf(me, cc, second ? other * sn : -other * sn);
+#pragma unroll
+            for (int k = 0; k < 2 * V; ++k)
+              if (k == e) x[k] = y;
+          }
+        }
+      } else if (turn && turns) {
         if (t.interleaved) {
 #pragma unroll
-          for (int j = 0; j < VPL; ++j)
-#pragma unroll
-            for (int e = 0; e < V; ++e) p[j][e] = x[j][e ^ 1];
-        } else if (lined) {
-          const int hv = half / V;
-#pragma unroll
-          for (int j = 0; j < VPL; ++j) {
-            const int vi = lane + j * GL;
-            const int pv = vi < hv ? vi + hv : (vi < 2 * hv ? vi - hv : vi);
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-              p[j][e] = __shfl_sync(KIV_FULL_MASK, x[0][e], pv % GL, GL);
-              if (VPL > 1) {
-                const float q1 = __shfl_sync(KIV_FULL_MASK, x[VPL - 1][e], pv % GL, GL);
-                if (pv >= GL) p[j][e] = q1;
-              }
+          for (int e = 0; e < V; ++e) {
+            const float p = x[2 * e], q = x[2 * e + 1];
+            if (e < V / 2 || vb * V < t.rot_dim) {
+              x[2 * e] = p * c[e] - q * s[e];
+              x[2 * e + 1] = q * c[e] + p * s[e];
             }
           }
         } else {
-          __syncwarp();
 #pragma unroll
-          for (int j = 0; j < VPL; ++j)
-#pragma unroll
-            for (int e = 0; e < V; ++e) s_row[grp][(lane + j * GL) * V + e] = x[j][e];
-          __syncwarp();
-#pragma unroll
-          for (int j = 0; j < VPL; ++j)
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-              const int xi = (lane + j * GL) * V + e;
-              const int pi = xi < half ? xi + half : (xi < 2 * half ? xi - half : xi);
-              p[j][e] = s_row[grp][pi];
-            }
-        }
-        if (turn) {
-#pragma unroll
-          for (int j = 0; j < VPL; ++j)
-#pragma unroll
-            for (int e = 0; e < V; ++e)
-              if ((lane + j * GL) * V + e < t.rot_dim) x[j][e] = x[j][e] * c[j][e] + p[j][e] * s[j][e];
+          for (int e = 0; e < V; ++e) {
+            const float p = x[e], q = x[V + e];
+            x[e] = p * c[e] - q * s[e];
+            x[V + e] = q * c[e] + p * s[e];
+          }
         }
       }
       if (poison && turn) {
 #pragma unroll
-        for (int j = 0; j < VPL; ++j)
-#pragma unroll
-          for (int e = 0; e < V; ++e) x[j][e] = __int_as_float(0x7fc00000);
+        for (int e = 0; e < 2 * V; ++e) x[e] = __int_as_float(0x7fc00000);
       }
       if (live && r < r_end) {
-        const int head = r - (which ? a.rows[0] : 0);
-        T *dst;
-        if (APPEND) {
-          dst = which == 0 ? static_cast<T *>(a.pc.k) + koff + head * a.pc.k_stride_h
-                           : static_cast<T *>(a.pc.v) + voff + head * a.pc.v_stride_h;
-        } else {
-          const kiv_rows &o = a.out[which];
-          dst = static_cast<T *>(o.p) + b * o.stride_b + head * o.stride_h + i * o.stride_t;
-        }
-#pragma unroll
-        for (int j = 0; j < VPL; ++j) {
-          const int vi = lane + j * GL;
-          if (vi < nv) st16(dst + vi * V, turn ? Elem<T>::pack(x[j]) : raw[u][j]);
-        }
+        T *row;
+        if (APPEND)
+          row = which == 0 ? dst[0] + r * a.pc.k_stride_h : dst[1] + (r - a.rows[0]) * a.pc.v_stride_h;
+        else
+          row = which == 0 ? dst[0] + r * a.out[0].stride_h : dst[1] + (r - a.rows[0]) * a.out[1].stride_h;
+        if (va < nv) st16(row + va * V, turn ? Elem<T>::pack(x) : ra[u]);
+        if (vb < nv) st16(row + vb * V, turn ? Elem<T>::pack(x + V) : rb[u]);
       }
     }
   }
@@ -338,35 +315,32 @@ __global__ void __launch_bounds__(RP_THREADS) turn_kernel(const __grid_constant_
 template <typename T, bool APPEND>
 static kiv_status launch_turn(TurnArgs a, int64_t tokens, cudaStream_t s) {
   constexpr int V = Elem<T>::V;
-  const int nv = a.head_dim / V;
+  const int lanes = (a.head_dim / V + 1) / 2;
   const int total = a.rows[0] + a.rows[1];
-  const int gl = nv <= 8 ? 8 : (nv <= 16 ? 16 : 32), groups = RP_THREADS / gl;
+  const int gl = lanes <= 4 ? 4 : lanes <= 8 ? 8 : lanes <= 16 ? 16 : 32, groups = RP_THREADS / gl;
   // Heads per group: many rows share a load of cos and sin, few keep the SMs
-  // filled -- about three blocks on each, down to one row per group, where the
-  // call is one chain of loads
-  a.hc = 8;
-  while (a.hc > 1 && tokens * ceil_div(total, a.hc) < (int64_t)3 * groups * sm_count()) a.hc /= 2;
-  a.nch = (int)ceil_div(total, a.hc);
-  a.ntok = tokens;
-  const int64_t blocks = ceil_div(tokens * a.nch, groups);
-  if (blocks > 0x7fffffff) {
-    set_error("too many rows for one call");
-    return KIV_ERR_UNSUPPORTED;
-  }
-  auto lines = [](const void *p, int dtype, int64_t per) {   // `per` values from p on, and from multiples of `per` on
-    const int64_t bytes = std::min<int64_t>(16, per * elem_bytes(dtype));
-    return reinterpret_cast<uintptr_t>(p) % bytes == 0;
+  // filled -- two blocks on each, down to one row per group, where the call is
+  // one chain of loads
+  a.hc = 16;
+  while (a.hc > 1 && ceil_div(tokens, groups) * ceil_div(total, a.hc) < (int64_t)2 * sm_count()) a.hc /= 2;
+  while (ceil_div(total, a.hc) > 65535) a.hc *= 2;
+  a.ntok = (uint32_t)tokens;
+  const dim3 grid((unsigned)ceil_div(tokens, groups), (unsigned)ceil_div(total, a.hc));
+  auto lines = [](const void *p, int dtype) {   // V values from p on, and from multiples of V on
+    return reinterpret_cast<uintptr_t>(p) % std::min<int64_t>(16, (int64_t)V * elem_bytes(dtype)) == 0;
   };
   const kiv_turn &t = a.t;
-  const int per_cs = t.interleaved ? V / 2 : V;
-  a.vec_cs = t.cos && lines(t.cos, t.cs_dtype, per_cs) && lines(t.sin, t.cs_dtype, per_cs) && t.cs_stride % per_cs == 0;
-  a.vec_w = (!t.q_weight || lines(t.q_weight, t.weight_dtype, V)) && (!t.k_weight || lines(t.k_weight, t.weight_dtype, V));
-  const dim3 grid((unsigned)blocks);
+  a.vec_cs = t.cos && lines(t.cos, t.cs_dtype) && lines(t.sin, t.cs_dtype) && t.cs_stride % V == 0;
+  a.vec_w = (!t.q_weight || lines(t.q_weight, t.weight_dtype)) && (!t.k_weight || lines(t.k_weight, t.weight_dtype));
   cudaError_t e;
-  if (gl == 8) e = launch_pdl(turn_kernel<T, 8, 1, APPEND>, grid, dim3(RP_THREADS), 0, s, 1, a);
-  else if (gl == 16) e = launch_pdl(turn_kernel<T, 16, 1, APPEND>, grid, dim3(RP_THREADS), 0, s, 1, a);
-  else if (nv <= 32) e = launch_pdl(turn_kernel<T, 32, 1, APPEND>, grid, dim3(RP_THREADS), 0, s, 1, a);
-  else e = launch_pdl(turn_kernel<T, 32, 2, APPEND>, grid, dim3(RP_THREADS), 0, s, 1, a);
+#define KIV_TURN(GL)                                                                                               \
+  (a.turned && t.norm ? launch_pdl(turn_kernel<T, GL, APPEND, true>, grid, dim3(RP_THREADS), 0, s, 1, a)           \
+                      : launch_pdl(turn_kernel<T, GL, APPEND, false>, grid, dim3(RP_THREADS), 0, s, 1, a))
+  if (gl == 4) e = KIV_TURN(4);
+  else if (gl == 8) e = KIV_TURN(8);
+  else if (gl == 16) e = KIV_TURN(16);
+  else e = KIV_TURN(32);
+#undef KIV_TURN
   return cuda_status(e, APPEND ? "paged_append" : "qk_norm_rope");
 }
 

@@ -409,3 +409,33 @@ def test_nothing_to_do():
     out = paged.paged_attend(c.q, *c.args(), 0.1)
     assert out.shape == (0, 4, 64)
     paged.paged_append(c.k, c.v, *c.args())
+
+
+def test_turn_by_sections_of_axes_and_mixed_pairs():
+    """Lanes whose pairs share an axis, lanes whose pairs do not, five axes, and an axis out of range."""
+    g = torch.Generator().manual_seed(5)
+    q = torch.randn(1, 3, 9, 128, generator=g).to(BF).to(DEV)
+    cos, sin = paged.rotary_table(1e4 ** (-torch.arange(64, dtype=torch.float64, device=DEV) / 64), 500)
+    pos = torch.randint(0, 500, (5, 1, 9), generator=g).to(DEV)
+    for pair in ([j // 13 for j in range(64)], [j // 16 for j in range(64)], [4 - j % 5 for j in range(64)], [4] * 64):
+        for inter in (False, True):
+            axes = torch.tensor(pair, dtype=torch.int32, device=DEV)
+            got, _ = paged.qk_norm_rope(q, None, cos, sin, positions=pos, pair_axes=axes, interleaved=inter)
+            at = pos[axes.long()].permute(1, 2, 0)
+            j = torch.arange(64, device=DEV)
+            want = ref_turn(q.double(), None, None, cos.double()[at, j][:, None], sin.double()[at, j][:, None], inter)
+            assert ((got.double() - want).abs() <= HALF[BF] * want.abs() + 1e-6 * want.abs().amax(-1, keepdim=True)).all()
+    axes = torch.zeros(64, dtype=torch.int32, device=DEV)
+    axes[7] = 5
+    err = torch.zeros(1, dtype=torch.int64, device=DEV)
+    got, _ = paged.qk_norm_rope(q, None, cos, sin, positions=pos, pair_axes=axes, errors=err)
+    assert got.isnan().all() and int(err) == nat.ERRBIT_POSITION
+
+
+def test_attend_windows_and_chunks_of_many_lengths_in_one_batch():
+    """Many items per block, most with dead rows at both ends of their keys, some of one row tile and some of two."""
+    new = [1021, 1, 300, 130, 64, 65, 700, 256, 33]
+    lens = [7000, 5, 300, 2000, 6001, 1999, 3333, 256, 4000]
+    for window, softcap in ((1500, 30.0), (200, 0.0), (0, 0.0)):
+        check_attend(Case(new, lens, 16, 16, 96, 48, HF, seed=1), window=window, softcap=softcap)
+        check_attend(Case(new[1:6], lens[1:6], 8, 1, 256, 24, BF, seed=2), window=window, softcap=softcap)
