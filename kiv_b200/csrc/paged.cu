@@ -188,11 +188,11 @@ __global__ void __launch_bounds__(CC_THREADS) paged_cc_kernel(const __grid_const
 #pragma unroll
         for (int w = 8; w > 0; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(KIV_FULL_MASK, mx, w));
         const float ms = mx == -INFINITY ? 0.f : mx;     // a row that has seen nothing yet: exp(-inf) = 0
-        const float keep = exp2f((m[a] - ms) * 1.44269504f);
+        const float keep = ex2((m[a] - ms) * 1.44269504f);
         float sum = 0.f;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          const float e = exp2f((s[a][c] - ms) * 1.44269504f);
+          const float e = ex2((s[a][c] - ms) * 1.44269504f);
           sp[(tr * RPT + a) * (CC_KEYS + 4) + tc + 16 * c] = e;
           sum += e;
         }
@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(CB_WARPS * 32) paged_combine_kernel(const __gr
 #pragma unroll 4
     for (int c = c0; c <= last; ++c) {
       const float *src = paged_part(p, 2 * (int64_t)c + (c == c0), r);
-      const float w = exp2f((src[D] - ms) * 1.44269504f);
+      const float w = ex2((src[D] - ms) * 1.44269504f);
       l = fmaf(src[D + 1], w, l);
       if (col < D) {
         const float4 v = *reinterpret_cast<const float4 *>(src + col);
@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(CB_WARPS * 32) paged_combine_kernel(const __gr
 kiv_status launch_paged_combine(const PagedPlan &p, int blocks, cudaStream_t s) {
   if (blocks < 2) return KIV_OK;
   const int slices = (int)ceil_div(p.pc.head_dim, 128);
-  const int y = (int)std::min<int64_t>(ceil_div((int64_t)p.tpt * p.grp * slices, CB_WARPS), 8);
+  const int y = (int)std::min<int64_t>(ceil_div((int64_t)p.tpt * p.grp * slices, CB_WARPS), 32);
   const dim3 grid((unsigned)blocks, (unsigned)y), block(CB_WARPS * 32);
   cudaError_t e;
   if (p.pc.dtype == KIV_DTYPE_F32) e = launch_pdl(paged_combine_kernel<float>, grid, block, 0, s, 1, p);
@@ -354,8 +354,6 @@ static PagedPlan make_plan(const kiv_paged *pc, const kiv_paged_query *q, int ro
   p.tpt = rows / p.grp;
   p.kt = kt;
   p.rows = rows;
-  p.min_tokens = 0;
-  p.max_tokens = 0x7fffffff;
   return p;
 }
 
@@ -369,61 +367,42 @@ struct PagedCall {
   size_t cut_offset;
 };
 
-static void size_call(PagedCall &c) {
-  c.cut_offset = (size_t)align_up((int64_t)2 * c.blocks * c.p.rows * partial_stride(c.p.pc.head_dim) * 4, 256);
-  c.bytes = c.cut_offset + (size_t)align_up((int64_t)c.blocks * sizeof(PagedCut), 256);
-}
-
-// Rows per key head from which a sequence's chunk goes to tcgen05
-constexpr int TC_ROWS = 65;
-
-// The kernels of a call (one or two) and their tilings.  The lengths are on
-// the device, so the host goes by what it knows: the number of rows, and
-// max_query_len.  Where that leaves both kinds of sequences possible, both
-// kernels run and each takes its own sequences.
-static int plan_calls(const kiv_paged *pc, const kiv_paged_query *q, PagedCall (&c)[2]) {
+// The kernel of a call and its tiling.  tcgen05 wherever TMA can bring the
+// pages (paged_tc.cu): for single tokens too, 210 us against 250 (64 x 16 k
+// keys of 32/8 x 128) and 62 against 84 (8/1 x 256) by the split kernel, which
+// keeps the pages of odd sizes and strides, the head dimensions 80 and 192 and
+// heads in groups above 128; CUDA cores for fp32 and what is left.  The lengths
+// are on the device, so the row tiles of the latter two go by what the host
+// knows: the rows of the longest sequence (max_query_len), or the mean.
+static PagedCall plan_call(const kiv_paged *pc, const kiv_paged_query *q) {
+  PagedCall c;
   const int D = pc->head_dim;
-  const int64_t per = q->num_query_heads / pc->num_kv_heads, T = pc->num_tokens, B = std::max(1, pc->batch);
-  const int64_t most = std::min<int64_t>(T, pc->max_query_len > 0 ? pc->max_query_len : T);   // tokens of one sequence
-  const int64_t mean = ceil_div(T, B);
-  const int64_t likely = per * std::min(most, pc->max_query_len > 0 ? most : mean);
-  if (!paged_mma_head(pc->dtype, D)) {
-    const int rows = likely <= 16 ? 16 : 64;
-    c[0].kernel = PAGED_CC;
-    c[0].p = make_plan(pc, q, rows, CC_KEYS);
-    const size_t smem = rows == 16 ? cc_smem<16>(D) : cc_smem<64>(D);
-    c[0].blocks = sm_count() * (int)std::max<size_t>(1, std::min<size_t>(4, (220 * 1024) / (smem + 2048)));
-    size_call(c[0]);
-    return 1;
-  }
-  // most * B == T: every sequence has `most` new tokens.  T <= B: single tokens.
-  const bool tc = paged_tc_eligible(pc, q);
-  const bool only_small = !tc || per * most < TC_ROWS || (T <= B && pc->max_query_len == 0);
-  const bool only_large = !only_small && most * B == T;
-  int n = 0;
-  if (!only_large) {
-    PagedCall &m = c[n++];
-    const int64_t at = only_small ? likely : per;
-    const int rows = at <= 16 ? 16 : at <= 32 ? 32 : 64;
-    m.kernel = PAGED_MMA;
-    m.p = make_plan(pc, q, rows, 64);
-    if (!only_small) m.p.max_tokens = (int)((TC_ROWS - 1) / per);
-    m.blocks = paged_mma_blocks(D, rows);
-    size_call(m);
-  }
-  if (!only_small) {
-    PagedCall &t = c[n++];
-    t.kernel = PAGED_TC;
-    t.p = make_plan(pc, q, 128, 128);
+  const int64_t per = q->num_query_heads / pc->num_kv_heads;
+  const int64_t mean = ceil_div(pc->num_tokens, std::max(1, pc->batch));
+  const int64_t likely = per * (pc->max_query_len > 0 ? std::min<int64_t>(pc->max_query_len, pc->num_tokens) : mean);
+  if (paged_tc_eligible(pc, q)) {
+    c.kernel = PAGED_TC;
+    c.p = make_plan(pc, q, 128, 128);
     if (D <= 128) {                 // two row tiles per item; at 256 TMEM holds the output of one
-      t.p.tpt *= 2;
-      t.p.rows = 256;
+      c.p.tpt *= 2;
+      c.p.rows = 256;
     }
-    if (!only_large) t.p.min_tokens = (int)((TC_ROWS - 1) / per) + 1;
-    t.blocks = sm_count();
-    size_call(t);
+    c.blocks = sm_count();
+  } else if (paged_mma_head(pc->dtype, D)) {
+    c.kernel = PAGED_MMA;
+    const int rows = likely <= 16 ? 16 : likely <= 32 ? 32 : 64;
+    c.p = make_plan(pc, q, rows, 64);
+    c.blocks = paged_mma_blocks(D, rows);
+  } else {
+    c.kernel = PAGED_CC;
+    const int rows = likely <= 16 ? 16 : 64;
+    c.p = make_plan(pc, q, rows, CC_KEYS);
+    const size_t smem = rows == 16 ? cc_smem<16>(D) : cc_smem<64>(D);
+    c.blocks = sm_count() * (int)std::max<size_t>(1, std::min<size_t>(4, (220 * 1024) / (smem + 2048)));
   }
-  return n;
+  c.cut_offset = (size_t)align_up((int64_t)2 * c.blocks * c.p.rows * partial_stride(D) * 4, 256);
+  c.bytes = c.cut_offset + (size_t)align_up((int64_t)c.blocks * sizeof(PagedCut), 256);
+  return c;
 }
 
 template <typename T, int R, int DM>
@@ -463,23 +442,19 @@ extern "C" {
 
 size_t kiv_paged_workspace_bytes(const kiv_paged *pc, const kiv_paged_query *q) {
   if (check_paged(pc) != KIV_OK || !q || q->num_query_heads < 1 || q->num_query_heads % pc->num_kv_heads || pc->head_dim > 256) return 0;
-  PagedCall c[2];
-  return plan_calls(pc, q, c) == 1 ? c[0].bytes : c[0].bytes + c[1].bytes;
+  return plan_call(pc, q).bytes;
 }
 
 kiv_status kiv_paged_attend(const kiv_paged *pc, const kiv_paged_query *q, void *ws, size_t ws_bytes, void *stream) {
   KIV_CHECK(check_paged(pc));
   KIV_CHECK(check_paged_query(pc, q));
   if (pc->num_tokens == 0 || pc->batch == 0) return KIV_OK;
-  PagedCall c[2];
-  const int n = plan_calls(pc, q, c);
-  const size_t need = n == 1 ? c[0].bytes : c[0].bytes + c[1].bytes;
-  if (!ws || ws_bytes < need || (reinterpret_cast<uintptr_t>(ws) & 255)) {
-    set_error("workspace too small or misaligned (%zu < %zu)", ws_bytes, need);
+  const PagedCall c = plan_call(pc, q);
+  if (!ws || ws_bytes < c.bytes || (reinterpret_cast<uintptr_t>(ws) & 255)) {
+    set_error("workspace too small or misaligned (%zu < %zu)", ws_bytes, c.bytes);
     return KIV_ERR_CAPACITY;
   }
-  KIV_CHECK(run_call(c[0], static_cast<char *>(ws), (cudaStream_t)stream));
-  return n == 1 ? KIV_OK : run_call(c[1], static_cast<char *>(ws) + c[0].bytes, (cudaStream_t)stream);
+  return run_call(c, static_cast<char *>(ws), (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -80,7 +80,6 @@ struct PagedPlan {
   int tpt;       // tokens per row tile
   int kt;        // keys per key tile
   int rows;      // rows per part in the workspace: tpt * grp <= rows
-  int min_tokens, max_tokens;   // takes the sequences whose new tokens' count is in this range
   float *part;   // [2 * G][rows][D + 2 (rounded to 4)]
   struct PagedCut *cut;     // [G]
 };
@@ -124,14 +123,14 @@ kiv_status launch_paged_tc(const PagedPlan &p, int blocks, cudaStream_t s);
 
 struct PagedItems {      // the items of one sequence
   PagedSeq s;
-  int nrt;               // row tiles (0: none of this kernel's)
+  int nrt;               // row tiles
   int base;              // place of new token 0 (causal), or the length
 };
 
 __device__ __forceinline__ PagedItems paged_items(const PagedPlan &p, int b) {
   PagedItems it;
   it.s = paged_seq(p.pc, b);
-  it.nrt = it.s.n > 0 && it.s.n >= p.min_tokens && it.s.n <= p.max_tokens ? (it.s.n + p.tpt - 1) / p.tpt : 0;
+  it.nrt = (it.s.n + p.tpt - 1) / p.tpt;
   it.base = p.q.causal ? it.s.len - it.s.n : it.s.len;
   return it;
 }
@@ -327,6 +326,46 @@ __device__ __forceinline__ bool paged_row(const PagedPlan &p, const PagedItems &
   const int gi = (hp % p.hs) * p.grp + g;
   head = (hp / p.hs) * per + gi;
   return ti < p.tpt && i < it.s.n && gi < per;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Capped scores: s <- cap * tanh(scaling * s / cap), N per lane of a converged
+// warp.  tanh(x) = 1 - 2 / (1 + e^2x) costs two special-function operations per
+// score, twice what the softmax itself does, so where no score of the warp
+// passes 0.7 of the cap an odd polynomial serves: x P(x^2), P the degree-5
+// Chebyshev fit of tanh(x) / x on [0, 0.49] (relative error 3e-8 in fp32).
+template <int N>
+__device__ __forceinline__ void cap_scores(float *s, float cap, float scaling) {
+  const float k = scaling / cap;
+  float most = 0.f;
+#pragma unroll
+  for (int x = 0; x < N; ++x) most = fmaxf(most, fabsf(s[x]));
+  if (__all_sync(KIV_FULL_MASK, most * fabsf(k) <= 0.7f)) {
+    const float2 k2 = make_float2(k, k), c2 = make_float2(scaling, scaling);
+#pragma unroll
+    for (int x = 0; x < N; x += 2) {
+      const float2 v = make_float2(s[x], s[x + 1]);
+      const float2 t = __fmul2_rn(v, k2), u = __fmul2_rn(t, t);
+      float2 y = make_float2(-0.005094828f, -0.005094828f);
+      y = __ffma2_rn(y, u, make_float2(0.020032447f, 0.020032447f));
+      y = __ffma2_rn(y, u, make_float2(-0.053529456f, -0.053529456f));
+      y = __ffma2_rn(y, u, make_float2(0.133284763f, 0.133284763f));
+      y = __ffma2_rn(y, u, make_float2(-0.333331347f, -0.333331347f));
+      y = __ffma2_rn(y, u, make_float2(1.f, 1.f));
+      y = __fmul2_rn(y, __fmul2_rn(v, c2));
+      s[x] = y.x;
+      s[x + 1] = y.y;
+    }
+  } else {
+    const float e = 2.f * 1.44269504f * k;
+#pragma unroll
+    for (int x = 0; x < N; ++x) s[x] = cap * (1.f - __fdividef(2.f, 1.f + ex2(s[x] * e)));
+  }
 }
 
 // Where a finished row goes

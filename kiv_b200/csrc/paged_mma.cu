@@ -235,13 +235,14 @@ __global__ void __launch_bounds__(MM_THREADS, MmaShape<D, 16 * WM>::BLOCKS) page
       }
       const int64_t j0 = j00 + (int64_t)t * MM_KEYS;
       const bool open = j0 >= free_lo && j0 + MM_KEYS - 1 <= free_hi;
+      const bool cap = p.q.softcap > 0.f;
+      if (cap) cap_scores<NK / 2>(&s[0][0], p.q.softcap, scale);
       float mx[2] = {m[0], m[1]};
 #pragma unroll
       for (int n = 0; n < NK / 8; ++n) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          float x = s[n][e] * scale;
-          if (p.q.softcap > 0.f) x = p.q.softcap * tanhf(x / p.q.softcap);
+          float x = cap ? s[n][e] : s[n][e] * scale;
           if (!open) {
             const int64_t j = j0 + wn * NK + n * 8 + 2 * tq + (e & 1);
             const int pl = place[e >> 1];
@@ -260,7 +261,7 @@ __global__ void __launch_bounds__(MM_THREADS, MmaShape<D, 16 * WM>::BLOCKS) page
         float keep[2];
 #pragma unroll
         for (int a = 0; a < 2; ++a) {
-          keep[a] = mx[a] == -INFINITY ? 1.f : exp2f((m[a] - mx[a]) * 1.44269504f);
+          keep[a] = mx[a] == -INFINITY ? 1.f : ex2((m[a] - mx[a]) * 1.44269504f);
           l[a] *= keep[a];
           m[a] = mx[a];
         }
@@ -277,7 +278,7 @@ __global__ void __launch_bounds__(MM_THREADS, MmaShape<D, 16 * WM>::BLOCKS) page
       for (int n = 0; n < NK / 8; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          s[n][e] = exp2f(fmaf(s[n][e], 1.44269504f, -ms[e >> 1]));
+          s[n][e] = ex2(fmaf(s[n][e], 1.44269504f, -ms[e >> 1]));
           l[e >> 1] += s[n][e];
         }
       const uint32_t vaddr = vt + (wn * NK + (lane & 15)) * S::LD + (lane >> 4) * 16;
@@ -341,7 +342,7 @@ __global__ void __launch_bounds__(MM_THREADS, MmaShape<D, 16 * WM>::BLOCKS) page
 #pragma unroll
       for (int w = 0; w < WN; ++w) {
         const float *row = sx + (w * ROWS + r) * XLD;
-        const float f = exp2f((row[D] - ms) * 1.44269504f);
+        const float f = ex2((row[D] - ms) * 1.44269504f);
         ll = fmaf(row[D + 1], f, ll);
 #pragma unroll
         for (int e = 0; e < 8; ++e) acc[e] = fmaf(row[c + e], f, acc[e]);

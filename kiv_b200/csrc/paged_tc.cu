@@ -11,6 +11,13 @@
 //            ring, one box of `br` rows per page piece;
 //   warps 9, 10  MMA of row tile 0 and 1: O += P(j) V(j), then S(j+1);
 //   warps 0-3 and 4-7: softmax of row tile 0 and 1, a thread per row.
+// An item with one row tile (a single token's heads, a few drafted tokens, a
+// short prompt) would leave one group idle and the other one's chain scores ->
+// softmax -> product exposed: there both take the same rows, one over the even
+// key tiles and one over the odd ones, and join at the end ("twins").  So the
+// same kernel serves decode, bound by memory: warps without rows only keep the
+// beat, and the tensor cores' empty rows cost nothing that is missed (CUDA-core
+// free m16n8k16 products took TWIN_CMP).
 // While one row tile's softmax runs, the tensor cores work on the other's
 // products, so both are kept busy: per tile pair the tensor cores need 4 x 512
 // cycles (D = 128) and the 2 x 16384 exponentials 2048 cycles of the special
@@ -55,6 +62,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
   __shared__ int64_t sm[40];
   __shared__ uint32_t s_tmem;
   __shared__ PtSeg seg[2];
+  __shared__ float s_ml[2][PT_ROWS];           // of the second of two twins
   // broadcast: the compiler then knows that a role's control flow is the warp's
   const int warp = __shfl_sync(KIV_FULL_MASK, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   uint8_t *smem = pt_dyn + ((1024 - (smem_u32(pt_dyn) & 1023)) & 1023);
@@ -164,7 +172,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
     constexpr uint32_t id_s = tc::idesc_f16(BF, PT_ROWS, PT_KEYS);
     constexpr uint32_t id_o = tc::idesc_f16(BF, PT_ROWS, D) | (1u << 16);     // B is MN-major
     constexpr uint32_t TILE16 = S::TILE >> 4;
-    const uint64_t qd = (S::BOX == 64 ? tc::sdesc_k128(smem_u32(qmem)) : tc::sdesc_k64(smem_u32(qmem))) + (uint32_t)i * TILE16;
+    const uint64_t qd = S::BOX == 64 ? tc::sdesc_k128(smem_u32(qmem)) : tc::sdesc_k64(smem_u32(qmem));
     const uint64_t kd = S::BOX == 64 ? tc::sdesc_k128(smem_u32(ring)) : tc::sdesc_k64(smem_u32(ring));
     const uint64_t vd = tc::sdesc_mn<S::BOXB>(smem_u32(ring), PT_KEYS * S::BOXB);
     const uint32_t ts = tmem + i * PT_KEYS, to = tmem + 2 * PT_KEYS + i * D;
@@ -180,49 +188,62 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
         phase ^= 1;
       }
     };
-    auto scores = [&]() {
+    auto scores = [&](uint64_t qa) {
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
         const uint32_t off = ((uint32_t)(k * 16 / S::BOX) * (PT_ROWS * S::BOXB) + (uint32_t)(k * 16 % S::BOX) * 2) >> 4;
-        tc::mma_f16(ts, qd + off, kd + slot * TILE16 + off, id_s, k > 0 ? 1u : 0u);
+        tc::mma_f16(ts, qa + off, kd + slot * TILE16 + off, id_s, k > 0 ? 1u : 0u);
       }
       tc::commit(&s_full[i]);
       tc::commit(&kv_empty[slot]);
+    };
+    auto pass = [&]() {                        // a tile that is the other warp's
+      wait(&kv_full[slot], phase);
+      __syncwarp();
+      if (leader) mbar_arrive(&kv_empty[slot]);
+      bump();
     };
     for (uint32_t items = 0;; ++items) {
       wait(&q_full, items & 1);
       const int ntile = __shfl_sync(KIV_FULL_MASK, ok ? seg[items & 1].ntile : 0, 0);
       const int nsub = __shfl_sync(KIV_FULL_MASK, seg[items & 1].nsub, 0);
+      const bool twin = nsub == 1 && ntile > 1;
       if (ntile == 0) break;
-      if (i >= nsub) {                         // no such row tile: only pass the ring on
+      if (i > 0 && nsub == 1 && !twin) {       // one tile of one row tile: nothing for this warp
         if (leader) mbar_arrive(&q_empty);
-        for (int t = 0; t < 2 * ntile; ++t) {
-          wait(&kv_full[slot], phase);
-          __syncwarp();
-          if (leader) mbar_arrive(&kv_empty[slot]);
-          bump();
-        }
+        pass();
+        pass();
         continue;
+      }
+      const int step = twin ? 2 : 1, first = twin ? i : 0;
+      const uint64_t qa = qd + (twin ? 0u : (uint32_t)i * TILE16);
+      if (first > 0) {
+        pass();
+        pass();
       }
       wait(&kv_full[slot], phase);
       tc::fence_after_sync();
       if (leader) {
-        scores();
-        if (ntile == 1) tc::commit(&q_empty);
+        scores(qa);
+        if (first + step >= ntile) tc::commit(&q_empty);
       }
       bump();
-      for (int t = 0; t < ntile; ++t, ++tiles) {
-        const bool more = t + 1 < ntile;
+      for (int t = first; t < ntile; t += step, ++tiles) {
+        const bool more = t + step < ntile;
         const uint32_t vs = slot;
         wait(&kv_full[vs], phase);
         bump();
+        if (twin && t + 1 < ntile) {
+          pass();
+          pass();
+        }
         if (more) wait(&kv_full[slot], phase);
         const uint64_t b = vd + vs * TILE16;
         wait(&p_full[i], tiles & 1);
         tc::fence_after_sync();
         if (leader) {
 #pragma unroll
-          for (int k = 0; k < PT_HEAD / 16; ++k) tc::mma_f16_ta(to, ts + k * 8, b + k * S::BOXB, id_o, (t > 0 || k > 0) ? 1u : 0u);
+          for (int k = 0; k < PT_HEAD / 16; ++k) tc::mma_f16_ta(to, ts + k * 8, b + k * S::BOXB, id_o, (t > first || k > 0) ? 1u : 0u);
         }
         wait(&p_tail[i], tiles & 1);
         tc::fence_after_sync();
@@ -230,9 +251,9 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
 #pragma unroll
           for (int k = PT_HEAD / 16; k < PT_KEYS / 16; ++k) tc::mma_f16_ta(to, ts + k * 8, b + k * S::BOXB, id_o, 1u);
           if (!more) tc::commit(&o_full[i]);
-          if (more) scores();
+          if (more) scores(qa);
           tc::commit(&kv_empty[vs]);
-          if (more && t + 2 == ntile) tc::commit(&q_empty);
+          if (more && t + 2 * step >= ntile) tc::commit(&q_empty);
         }
         if (more) bump();
       }
@@ -241,12 +262,11 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
   } else {
     // ------------------------------------------------ softmax of row tile `sub`
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PT_REGS_SOFTMAX));
-    const int sub = warp >> 2, r = (warp & 3) * 32 + lane;
+    const int grp = warp >> 2, r = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t ts = tmem + lanes + sub * PT_KEYS, to = tmem + lanes + 2 * PT_KEYS + sub * D;
+    const uint32_t ts = tmem + lanes + grp * PT_KEYS, to = tmem + lanes + 2 * PT_KEYS + grp * D;
     const bool cap = p.q.softcap > 0.f;
     const float c = (cap ? 1.f : p.q.scaling) * 1.44269504f;              // scores are powers of two of s c
-    const float cap_in = cap ? 2.f * 1.44269504f * p.q.scaling / p.q.softcap : 0.f;
     const int ti = r / p.grp, gi = r - ti * p.grp;
     uint32_t tiles = 0, outs = 0, next = 0, before;   // before: tiles of the block's earlier segments
     for (uint32_t items = 0;; ++items) {
@@ -256,8 +276,16 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
       next += w.ntile;
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_empty);
-      if (!ok || w.ntile == 0) break;
-      if (sub >= w.nsub) continue;
+      // a wait that ran out in one warp ends the loop in all: they share barriers
+      uint32_t failed;
+      asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 q, %1, 0;\n bar.red.or.pred p, 1, 256, q;\n selp.u32 %0, 1, 0, p;\n}\n"
+                   : "=r"(failed)
+                   : "r"(ok ? 0u : 1u)
+                   : "memory");
+      if (failed || w.ntile == 0) break;
+      const bool twin = w.nsub == 1 && w.ntile > 1;
+      if (grp >= w.nsub && !twin) continue;
+      const int step = twin ? 2 : 1, first = twin ? grp : 0, sub = twin ? 0 : grp;   // sub: the row tile
       const int tok = sub * g.tps + ti;
       const bool have = ti < g.tps && gi < w.heads && tok < w.tok;
       const int place = p.q.causal ? w.base + tok : 0x7fffffff;
@@ -265,21 +293,40 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
       const int64_t t0 = (int64_t)w.base + sub * g.tps;
       const int64_t free_hi = p.q.causal ? min((int64_t)w.hi - 1, t0) : (int64_t)w.hi - 1;
       const int64_t free_lo = max((int64_t)w.lo, p.q.window > 0 ? t0 + g.tps - p.q.window : (int64_t)0);
+      const bool idle = (warp & 3) * 32 >= min(rows, (w.tok - sub * g.tps) * p.grp);   // a warp without rows keeps the beat
       float m = -INFINITY, l = 0.f;
-      for (int t = 0; t < w.ntile; ++t, ++tiles) {
-        if (ok && !mbar_wait_bounded(&s_full[sub], tiles & 1)) ok = false;
+      for (int t = first; t < w.ntile; t += step, ++tiles) {
+        if (ok && !mbar_wait_bounded(&s_full[grp], tiles & 1)) ok = false;
         tc::fence_after_sync();
+        const int64_t j0 = w.j00 + (int64_t)t * PT_KEYS;
+        if (j0 < w.lo || j0 + PT_KEYS > w.hi) {
+          // Dead rows of the V tile: each group clears them for its own
+          // product, which waits for p_full below.
+          const uint32_t n = 2 * (before + t) + 1, vs = n % SLOTS;
+          if (ok && !mbar_wait_bounded(&kv_full[vs], (n / SLOTS) & 1)) ok = false;
+          const int dl = (int)max((int64_t)0, w.lo - j0), dh = (int)max((int64_t)0, min((int64_t)PT_KEYS, w.hi - j0));
+          if (r < dl || r >= dh) {
+#pragma unroll 1
+            for (int y = 0; y < D / 8; ++y)
+              *reinterpret_cast<uint4 *>(ring + vs * S::TILE + (y / (S::BOX / 8)) * (PT_KEYS * S::BOXB) + r * S::BOXB +
+                                         (y % (S::BOX / 8)) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          tc::fence_proxy_async_smem();
+        }
+        if (idle) {                            // what P holds for these rows stays in their own rows
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&p_full[grp]);
+            mbar_arrive(&p_tail[grp]);
+          }
+          continue;
+        }
         uint32_t su[PT_KEYS];
 #pragma unroll
         for (int x = 0; x < PT_KEYS; x += 32) tc::ld_32x32(ts + x, su + x);
 #pragma unroll
         for (int x = 0; x < PT_KEYS; x += 32) tc::wait_ld32(su + x);
-        if (cap) {
-#pragma unroll
-          for (int x = 0; x < PT_KEYS; ++x)
-            su[x] = __float_as_uint(p.q.softcap * (1.f - __fdividef(2.f, 1.f + ex2(__uint_as_float(su[x]) * cap_in))));
-        }
-        const int64_t j0 = w.j00 + (int64_t)t * PT_KEYS;
+        if (cap) cap_scores<PT_KEYS>(reinterpret_cast<float *>(su), p.q.softcap, p.q.scaling);
         if (j0 < free_lo || j0 + PT_KEYS - 1 > free_hi) {
           // columns [bot, top] are seen
           const int top = (int)min((int64_t)PT_KEYS, min((int64_t)w.hi - 1, (int64_t)place) - j0);
@@ -287,20 +334,6 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
 #pragma unroll
           for (int x = 0; x < PT_KEYS; ++x)
             if (x > top || x < bot) su[x] = 0xff800000u;
-          if (j0 < w.lo || j0 + PT_KEYS > w.hi) {
-            // Dead rows of the V tile: each group clears them for its own
-            // product, which waits for p_full below.
-            const uint32_t n = 2 * (before + t) + 1, vs = n % SLOTS;
-            if (ok && !mbar_wait_bounded(&kv_full[vs], (n / SLOTS) & 1)) ok = false;
-            const int dl = (int)max((int64_t)0, w.lo - j0), dh = (int)max((int64_t)0, min((int64_t)PT_KEYS, w.hi - j0));
-            if (r < dl || r >= dh) {
-#pragma unroll 1
-              for (int y = 0; y < D / 8; ++y)
-                *reinterpret_cast<uint4 *>(ring + vs * S::TILE + (y / (S::BOX / 8)) * (PT_KEYS * S::BOXB) + r * S::BOXB +
-                                           (y % (S::BOX / 8)) * 16) = make_uint4(0, 0, 0, 0);
-            }
-            tc::fence_proxy_async_smem();
-          }
         }
         float mx[8];
 #pragma unroll
@@ -312,7 +345,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
             mx[y] = fmaxf(mx[y], fmaxf(__uint_as_float(su[x + 2 * y]), __uint_as_float(su[x + 2 * y + 1])));
         }
         const float mn = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])));
-        if (t == 0) {
+        if (t == first) {
           m = mn;
         } else if (__any_sync(KIV_FULL_MASK, (mn - m) * c > PT_LAZY)) {   // (-inf) - (-inf) is NaN: no growth
           const float f = mn == -INFINITY ? 1.f : ex2((m - mn) * c);
@@ -348,53 +381,86 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
             tc::wait_st();
             tc::fence_before_sync();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[sub]);
+            if (lane == 0) mbar_arrive(&p_full[grp]);
           }
         }
         l += (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y);
         tc::wait_st();
         tc::fence_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_tail[sub]);
+        if (lane == 0) mbar_arrive(&p_tail[grp]);
       }
       // ---- the item's rows
-      if (ok && !mbar_wait_bounded(&o_full[sub], outs & 1)) ok = false;
+      if (ok && !mbar_wait_bounded(&o_full[grp], outs & 1)) ok = false;
       ++outs;
       tc::fence_after_sync();
+      // Twins: two groups hold the same rows, over the even and the odd key
+      // tiles.  The second leaves maximum and sum in shared memory and its
+      // output in TMEM, where the first one's threads reach the same lanes.
+      float f0 = 1.f, f1 = 0.f;
+      if (twin) {
+        if (grp == 1) {
+          s_ml[0][r] = m;
+          s_ml[1][r] = l;
+          tc::fence_before_sync();
+          asm volatile("bar.sync 1, 256;" ::: "memory");
+          asm volatile("bar.sync 1, 256;" ::: "memory");     // read: the next item may overwrite it
+          tc::fence_after_sync();
+          continue;
+        }
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        tc::fence_after_sync();
+        const float m1 = s_ml[0][r], l1 = s_ml[1][r], top = fmaxf(m, m1);
+        f0 = m == -INFINITY ? 0.f : ex2((m - top) * c);
+        f1 = m1 == -INFINITY ? 0.f : ex2((m1 - top) * c);
+        m = top;
+        l = l * f0 + l1 * f1;
+      }
       const float mnat = m * c * 0.693147181f;
       const bool whole = w.part < 0;
-      const float inv = l > 0.f ? 1.f / l : 0.f;
+      const float inv = whole ? (l > 0.f ? 1.f / l : 0.f) : 1.f;
+      f0 *= inv;
+      f1 *= inv;
       const int head = w.head0 + gi;
       T *dst = static_cast<T *>(p.q.out) + (w.q0 + tok) * p.q.out_stride_t + head * p.q.out_stride_h;
       float *part = paged_part(p, w.part, sub * rows + r);
+      if (!idle) {
+#pragma unroll 1
+        for (int x = 0; x < D; x += 32) {
+          uint32_t o[32];
+          tc::ld_32x32(to + x, o);
+          tc::wait_ld32(o);
+          float *of = reinterpret_cast<float *>(o);
 #pragma unroll
-      for (int x = 0; x < D; x += 32) {
-        uint32_t o[32];
-        tc::ld_32x32(to + x, o);
-        tc::wait_ld32(o);
-        if (!have) continue;
-        if (whole) {
+          for (int y = 0; y < 32; ++y) of[y] = f0 == 0.f ? 0.f : of[y] * f0;   // nothing seen: what is there does not count
+          if (twin) {
+            uint32_t o1[32];
+            tc::ld_32x32(to + D + x, o1);
+            tc::wait_ld32(o1);
 #pragma unroll
-          for (int y = 0; y < 32; y += 8) {
-            uint4 u;
-            u.x = pt_pack<BF>(__uint_as_float(o[y]) * inv, __uint_as_float(o[y + 1]) * inv);
-            u.y = pt_pack<BF>(__uint_as_float(o[y + 2]) * inv, __uint_as_float(o[y + 3]) * inv);
-            u.z = pt_pack<BF>(__uint_as_float(o[y + 4]) * inv, __uint_as_float(o[y + 5]) * inv);
-            u.w = pt_pack<BF>(__uint_as_float(o[y + 6]) * inv, __uint_as_float(o[y + 7]) * inv);
-            st16(dst + x + y, u);
+            for (int y = 0; y < 32; ++y) of[y] = f1 == 0.f ? of[y] : fmaf(__uint_as_float(o1[y]), f1, of[y]);
           }
-        } else {
+          if (!have) continue;
+          if (whole) {
 #pragma unroll
-          for (int y = 0; y < 32; y += 4) st16(part + x + y, make_uint4(o[y], o[y + 1], o[y + 2], o[y + 3]));
+            for (int y = 0; y < 32; y += 8) st16(dst + x + y, Elem<T>::pack(of + y));
+          } else {
+#pragma unroll
+            for (int y = 0; y < 32; y += 4) st16(part + x + y, make_uint4(o[y], o[y + 1], o[y + 2], o[y + 3]));
+          }
+        }
+        if (have) {
+          if (whole) {
+            if (p.q.lse) p.q.lse[(w.q0 + tok) * p.q.num_query_heads + head] = l > 0.f ? mnat + logf(l) : -INFINITY;
+          } else {
+            part[D] = mnat;
+            part[D + 1] = l;
+          }
         }
       }
-      if (have) {
-        if (whole) {
-          if (p.q.lse) p.q.lse[(w.q0 + tok) * p.q.num_query_heads + head] = l > 0.f ? mnat + logf(l) : -INFINITY;
-        } else {
-          part[D] = mnat;
-          part[D + 1] = l;
-        }
+      if (twin) {
+        tc::fence_before_sync();
+        asm volatile("bar.sync 1, 256;" ::: "memory");
       }
       tc::fence_before_sync();                 // the next item's products overwrite the output
     }

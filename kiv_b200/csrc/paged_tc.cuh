@@ -96,12 +96,6 @@ __device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, i
 }
 }  // namespace tc
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // one lane of the (converged) warp
 __device__ __forceinline__ bool elect_one() {
   uint32_t p;

@@ -247,7 +247,6 @@ paged_tc256_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
     const uint32_t to = tmem + lanes + 2 * PT_KEYS + w * (P2_D / 2);     // this thread's half of the output row
     const bool cap = p.q.softcap > 0.f;
     const float c = (cap ? 1.f : p.q.scaling) * 1.44269504f;
-    const float cap_in = cap ? 2.f * 1.44269504f * p.q.scaling / p.q.softcap : 0.f;
     const int ti = r / p.grp, gi = r - ti * p.grp;
     P2Ring vr;
     uint32_t tiles = 0;
@@ -267,6 +266,7 @@ paged_tc256_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
       const int place = p.q.causal ? sg.base + ti : 0x7fffffff;
       const int64_t free_hi = p.q.causal ? min((int64_t)sg.hi - 1, (int64_t)sg.base) : (int64_t)sg.hi - 1;
       const int64_t free_lo = max((int64_t)sg.lo, p.q.window > 0 ? (int64_t)sg.base + g.tps - p.q.window : (int64_t)0);
+      const bool idle = (warp & 3) * 32 >= min(rows, sg.tok * p.grp);   // a warp without rows keeps the beat
       float m = -INFINITY, l = 0.f;
       vr.skip();                               // K(0)
       for (int t = 0; t < sg.ntile; ++t, ++tiles) {
@@ -274,17 +274,35 @@ paged_tc256_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         const uint32_t ts = tmem + lanes + (tiles & 1) * PT_KEYS;
         wait(&s_full[tiles & 1], (tiles >> 1) & 1);
         tc::fence_after_sync();
+        const int64_t j0 = sg.j00 + (int64_t)t * PT_KEYS;
+        if (j0 < sg.lo || j0 + PT_KEYS > sg.hi) {
+          // Dead rows of V half w, after the product before this one (which
+          // used the slot's turn before) and before this one's, which waits
+          // for p_full below.
+          if (tiles > 0) wait(&pv_done[(tiles - 1) & 1], ((tiles - 1) >> 1) & 1);
+          wait(&kv_full[vr.slot(w)], vr.parity(w));
+          const int dl = (int)max((int64_t)0, sg.lo - j0), dh = (int)max((int64_t)0, min((int64_t)PT_KEYS, sg.hi - j0));
+          const int row = w * 64 + (r >> 1);
+          if (row < dl || row >= dh) {
+#pragma unroll 1
+            for (int y = (r & 1) * 16; y < (r & 1) * 16 + 16; ++y)
+              *reinterpret_cast<uint4 *>(ring + vr.slot(w) * P2_SLOT + (y / 8) * (64 * 128) + (r >> 1) * 128 + (y % 8) * 16) =
+                  make_uint4(0, 0, 0, 0);
+          }
+          tc::fence_proxy_async_smem();
+        }
+        vr.skip();
+        if (idle) {                            // what P holds for these rows stays in their own rows
+          asm volatile("bar.sync 1, 256;" ::: "memory");
+          if (lane == 0) mbar_arrive(&p_full[tiles & 1]);
+          continue;
+        }
         uint32_t su[COLS];
         tc::ld_32x32(ts + w * COLS, su);
         tc::ld_32x32(ts + w * COLS + 32, su + 32);
         tc::wait_ld32(su);
         tc::wait_ld32(su + 32);
-        if (cap) {
-#pragma unroll
-          for (int x = 0; x < COLS; ++x)
-            su[x] = __float_as_uint(p.q.softcap * (1.f - __fdividef(2.f, 1.f + ex2(__uint_as_float(su[x]) * cap_in))));
-        }
-        const int64_t j0 = sg.j00 + (int64_t)t * PT_KEYS;
+        if (cap) cap_scores<COLS>(reinterpret_cast<float *>(su), p.q.softcap, p.q.scaling);
         if (j0 < free_lo || j0 + PT_KEYS - 1 > free_hi) {
           // of this thread's columns [bot, top] are seen
           const int top = (int)min((int64_t)PT_KEYS, min((int64_t)sg.hi - 1, (int64_t)place) - j0) - w * COLS;
@@ -292,24 +310,7 @@ paged_tc256_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
 #pragma unroll
           for (int x = 0; x < COLS; ++x)
             if (x > top || x < bot) su[x] = 0xff800000u;
-          if (j0 < sg.lo || j0 + PT_KEYS > sg.hi) {
-            // Dead rows of V half w, after the product before this one (which
-            // used the slot's turn before) and before this one's, which waits
-            // for p_full below.
-            if (tiles > 0) wait(&pv_done[(tiles - 1) & 1], ((tiles - 1) >> 1) & 1);
-            wait(&kv_full[vr.slot(w)], vr.parity(w));
-            const int dl = (int)max((int64_t)0, sg.lo - j0), dh = (int)max((int64_t)0, min((int64_t)PT_KEYS, sg.hi - j0));
-            const int row = w * 64 + (r >> 1);
-            if (row < dl || row >= dh) {
-#pragma unroll 1
-              for (int y = (r & 1) * 16; y < (r & 1) * 16 + 16; ++y)
-                *reinterpret_cast<uint4 *>(ring + vr.slot(w) * P2_SLOT + (y / 8) * (64 * 128) + (r >> 1) * 128 + (y % 8) * 16) =
-                    make_uint4(0, 0, 0, 0);
-            }
-            tc::fence_proxy_async_smem();
-          }
         }
-        vr.skip();
         float mx[4] = {m, m, m, m};
 #pragma unroll
         for (int x = 0; x < COLS; x += 8) {
