@@ -91,19 +91,23 @@ struct PagedCut {
   int64_t blocks;           // blocks that took part
 };
 
-__host__ __device__ inline int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
-  // sum over i < n of floor((a i + b) / m), a and b not negative: lattice
-  // points under a line, counted by exchanging the axes (Euclid's steps)
+// sum over i < n of floor((a i + b) / m), a and b not negative: lattice points
+// under a line, counted by exchanging the axes (Euclid's steps).  a n + b stays
+// below 2^32 here (places of tokens), so the divisions have 32 bits.
+__host__ __device__ inline int64_t floor_sum(int64_t count, uint32_t m, uint32_t a, int64_t b64) {
   int64_t ans = 0;
-  while (n > 0) {
-    ans += (n * (n - 1) / 2) * (a / m) + n * (b / m);
-    a %= m;
-    b %= m;
-    const int64_t y = a * n + b;
+  if (count <= 0) return 0;
+  uint32_t n = (uint32_t)count, b = (uint32_t)b64;
+  for (;;) {
+    const uint32_t qa = a / m, qb = b / m;
+    ans += (int64_t)((uint64_t)n * (n - 1) / 2) * qa + (int64_t)n * qb;
+    a -= qa * m;
+    b -= qb * m;
+    const uint32_t y = a * n + b;
     if (y < m) break;
     n = y / m;
-    b = y % m;
-    const int64_t x = a;
+    b = y - n * m;
+    const uint32_t x = a;
     a = m;
     m = x;
   }
@@ -168,7 +172,8 @@ __host__ __device__ inline int64_t paged_prefix(const PagedPlan &p, const PagedI
   // the last row tile may end at the length, the others end at whole tiles of tokens
   int64_t r = 0;
   if (x == it.nrt) r = paged_tiles(p, it, --x);
-  const int64_t t = p.tpt, k = p.kt, base = it.base;
+  const int64_t base = it.base;
+  const uint32_t t = p.tpt, k = p.kt;
   const int64_t k0 = base >= 1 ? 0 : min((int64_t)x, (1 - base) / t);   // row tiles with hi = 1
   r += k0 + floor_sum(x - k0, k, t, base + (k0 + 1) * t + k - 1);
   if (p.q.window > 0) {
@@ -254,10 +259,13 @@ __device__ __forceinline__ PagedSpot paged_locate(const PagedPlan &p, int64_t *s
   const int64_t per_head = paged_prefix(p, r.it, r.it.nrt);
   r.hp = (int)(rem / per_head);
   rem -= (int64_t)r.hp * per_head;
-  int a = 0, z = r.it.nrt;                       // largest rt with prefix(rt) <= rem
+  // largest rt with prefix(rt) <= rem: the lanes try 32 places at a time
+  int a = 0, z = r.it.nrt;
   while (z - a > 1) {
-    const int m = (a + z) / 2;
-    if (paged_prefix(p, r.it, m) <= rem) a = m; else z = m;
+    const int stride = (z - a + 31) / 32, x = a + lane * stride;
+    const unsigned under = __ballot_sync(KIV_FULL_MASK, x < z && paged_prefix(p, r.it, x) <= rem);
+    a += (31 - __clz(under)) * stride;           // lane 0 always holds
+    z = min(z, a + stride);
   }
   r.rt = a;
   r.off = rem - paged_prefix(p, r.it, a);

@@ -7,7 +7,7 @@
 // A block takes items of two row tiles of 128 rows: a row is (token, query
 // head of the key head), so the heads of a group share every K and V tile
 // (`tps` = 128 / heads whole tokens per tile).  Warp roles:
-//   warp 8   TMA: the query tiles, then K and V tiles of 128 keys through a
+//   warps 8, 11  TMA: the query tiles, then K and V tiles of 128 keys through a
 //            ring, one box of `br` rows per page piece;
 //   warps 9, 10  MMA of row tile 0 and 1: O += P(j) V(j), then S(j+1);
 //   warps 0-3 and 4-7: softmax of row tile 0 and 1, a thread per row.
@@ -106,8 +106,12 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
   const int rows = g.tps * p.grp;              // of a row tile
   if (warp >= 8) {
    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PT_REGS_OTHER));
-   if (warp == 8) {
+   if (warp == 8 || warp == 11) {
     // ------------------------------------------------ TMA
+    // Two warps share the boxes of every tile: with pages of 16 tokens a tile
+    // is 16 copies, and one warp issued them at 5.0 TB/s, no faster.
+    const int me = warp == 8 ? 0 : 1;
+    const bool leader = elect_one();
     uint32_t n = 0, items = 0;
     for (;; ++items) {
       const bool live = at.it.s.b >= 0 && at.unit < at.end;
@@ -115,8 +119,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
       PagedSegment cut = {};
       int kvh = 0;
       if (live) sg = pt_segment(p, at, g.tps, cut, kvh);
-      if (items > 0 && ok && !mbar_wait_bounded(&q_empty, (items - 1) & 1)) ok = false;
-      if (lane == 0) {
+      if (me == 0 && items > 0 && ok && !mbar_wait_bounded(&q_empty, (items - 1) & 1)) ok = false;
+      if (me == 0 && lane == 0) {
         seg[items & 1] = sg;
         if (!live) {
           mbar_arrive(&q_full);
@@ -148,12 +152,15 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
         for (int kv = 0; kv < 2; ++kv, ++n) {
           const uint32_t s = n % SLOTS;
           if (n >= SLOTS && ok && !mbar_wait_bounded(&kv_empty[s], (n / SLOTS - 1) & 1)) ok = false;
-          if (lane == 0) mbar_arrive_tx(&kv_full[s], S::TILE);
           __syncwarp();
-          if (lane < nbox)
-            for (int c = 0; c < S::NB; ++c)
-              tc::tma_load_4d(ring + s * S::TILE + c * (PT_KEYS * S::BOXB) + lane * g.br * S::BOXB, kv ? &vmap : &kmap, c * S::BOX,
-                              rw, kvh, pg, &kv_full[s]);
+          if (me == 0 && leader) mbar_arrive_tx(&kv_full[s], S::TILE);
+          const CUtensorMap *map = kv ? &vmap : &kmap;
+          for (int x = me; x < nbox * S::NB; x += 2) {      // box x / NB, columns x % NB
+            const int l = x / S::NB, c = x % S::NB;
+            const int32_t bp = __shfl_sync(KIV_FULL_MASK, pg, l), br = __shfl_sync(KIV_FULL_MASK, rw, l);
+            if (leader)
+              tc::tma_load_4d(ring + s * S::TILE + c * (PT_KEYS * S::BOXB) + l * g.br * S::BOXB, map, c * S::BOX, br, kvh, bp, &kv_full[s]);
+          }
         }
       }
       at.unit += sg.ntile;

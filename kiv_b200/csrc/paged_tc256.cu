@@ -4,7 +4,7 @@
 // one row tile and the two halves of the other 256 columns hold the scores of
 // two key tiles in turn: S(j+1) is computed while the softmax works on S(j).
 // Warp roles:
-//   warp 8   TMA: the query tile, then K and V of 128 keys through a ring of
+//   warps 8, 11  TMA: the query tile, then K and V of 128 keys through a ring of
 //            five 32 KB slots (K: two halves of the columns, V: two halves of
 //            the rows, so that every product finds its operand at one stride);
 //   warp 9   S(j+1) = Q K^T;    warp 10   O += P(j) V(j);
@@ -91,8 +91,10 @@ paged_tc256_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
 
   if (warp >= 8) {
    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PT_REGS_OTHER));
-   if (warp == 8) {
-    // ------------------------------------------------ TMA
+   if (warp == 8 || warp == 11) {
+    // ------------------------------------------------ TMA (two warps share the boxes of every slot)
+    const int me = warp == 8 ? 0 : 1;
+    const bool leader = elect_one();
     P2Ring r;
     const int nbox = PT_KEYS / g.br, half = 64 / g.br;    // boxes of a K tile; of a V half
     for (uint32_t items = 0;; ++items) {
@@ -101,8 +103,8 @@ paged_tc256_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
       PagedSegment cut = {};
       int kvh = 0;
       if (live) sg = pt_segment(p, at, g.tps, cut, kvh);
-      if (items > 0) wait(&q_empty, (items - 1) & 1);
-      if (lane == 0) {
+      if (me == 0 && items > 0) wait(&q_empty, (items - 1) & 1);
+      if (me == 0 && lane == 0) {
         seg[items & 1] = sg;
         if (!live) {
           mbar_arrive(&q_full);
@@ -125,25 +127,30 @@ paged_tc256_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
       };
       auto begin = [&](uint32_t h) {
         if (r.n + h >= P2_SLOTS) wait(&kv_empty[r.slot(h)], r.parity(h) ^ 1);
-        if (lane == 0) mbar_arrive_tx(&kv_full[r.slot(h)], P2_SLOT);
         __syncwarp();
+        if (me == 0 && leader) mbar_arrive_tx(&kv_full[r.slot(h)], P2_SLOT);
         return ring + r.slot(h) * P2_SLOT;
       };
-      auto load_k = [&](int32_t page, int32_t row) {
+      auto load_k = [&](int32_t page, int32_t row) {   // slot h: columns [128 h, 128 h + 128) of all rows
         for (uint32_t h = 0; h < 2; ++h) {
           uint8_t *dst = begin(h);
-          if (lane < nbox)
-            for (int c = 0; c < 2; ++c)
-              tc::tma_load_4d(dst + c * (PT_KEYS * 128) + lane * g.br * 128, &kmap, (2 * h + c) * 64, row, kvh, page, &kv_full[r.slot(h)]);
+          for (int l = 0; l < nbox; ++l) {
+            const int32_t bp = __shfl_sync(KIV_FULL_MASK, page, l), br = __shfl_sync(KIV_FULL_MASK, row, l);
+            if (leader) tc::tma_load_4d(dst + me * (PT_KEYS * 128) + l * g.br * 128, &kmap, (2 * h + me) * 64, br, kvh, bp, &kv_full[r.slot(h)]);
+          }
         }
         r.skip();
       };
-      auto load_v = [&](int32_t page, int32_t row) {
+      auto load_v = [&](int32_t page, int32_t row) {   // slot h: rows [64 h, 64 h + 64)
         for (uint32_t h = 0; h < 2; ++h) {
           uint8_t *dst = begin(h);
-          if (lane >= (int)h * half && lane < ((int)h + 1) * half)
-            for (int c = 0; c < 4; ++c)
-              tc::tma_load_4d(dst + c * (64 * 128) + (lane - h * half) * g.br * 128, &vmap, c * 64, row, kvh, page, &kv_full[r.slot(h)]);
+          for (int l = 0; l < half; ++l) {
+            const int32_t bp = __shfl_sync(KIV_FULL_MASK, page, h * half + l), br = __shfl_sync(KIV_FULL_MASK, row, h * half + l);
+            if (leader) {
+              for (int c = 2 * me; c < 2 * me + 2; ++c)
+                tc::tma_load_4d(dst + c * (64 * 128) + l * g.br * 128, &vmap, c * 64, br, kvh, bp, &kv_full[r.slot(h)]);
+            }
+          }
         }
         r.skip();
       };
