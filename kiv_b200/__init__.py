@@ -11,7 +11,7 @@ from .config import KIVConfig
 from .model_topology import ModelTopology
 
 __all__ = ["KIVConfig", "ColdKVStore", "ModelTopology", "detect_topology", "TieredKVCache",
-           "KIVMiddleware"]
+           "KIVMiddleware", "PagedKVCache"]
 
 
 def __getattr__(name: str):
@@ -27,4 +27,7 @@ def __getattr__(name: str):
     if name == "KIVMiddleware":
         from .middleware import KIVMiddleware
         return KIVMiddleware
+    if name == "PagedKVCache":
+        from .paged import PagedKVCache
+        return PagedKVCache
     raise AttributeError(f"module 'kiv_b200' has no attribute {name!r}")

@@ -15,9 +15,11 @@ the original attention function, exactly as the reference does.
 
 from __future__ import annotations
 
+import functools
 import importlib
 import inspect
 import logging
+import sys
 from typing import Any
 
 import torch
@@ -114,6 +116,66 @@ def hot_mask_for_kernel(attention_mask: torch.Tensor | None, hot_len: int, q_len
     return m, causal
 
 
+def _turns_half_split(fn: Any, head_dim: int) -> bool:
+    """Whether ``fn(q, k, cos, sin)`` turns pairs (j, j + head_dim / 2) by cos and sin, seen on a small CPU input."""
+    g = torch.Generator().manual_seed(0)
+    half = head_dim // 2
+    q, k = torch.randn(1, 2, 3, head_dim, generator=g), torch.randn(1, 1, 3, head_dim, generator=g)
+    c, s = torch.randn(1, 3, half, generator=g), torch.randn(1, 3, half, generator=g)
+    try:
+        got = fn(q, k, torch.cat([c, c], -1), torch.cat([s, s], -1))
+        for x, y in zip((q, k), got):
+            a, b = x[..., :half], x[..., half:]
+            want = torch.cat([a * c - b * s, b * c + a * s], -1)
+            if y.shape != want.shape or not torch.allclose(y, want, rtol=1e-5, atol=1e-5):
+                return False
+        return len(got) == 2
+    except Exception:
+        return False
+
+
+def _repeats_halves(rotary: Any, device: torch.device) -> bool:
+    """Whether the model's rotary module gives each pair's cos and sin twice, ``cat([f, f], -1)``."""
+    try:
+        with torch.no_grad():
+            cos, sin = rotary(torch.zeros(1, 3, 8, device=device), torch.arange(3, device=device)[None])
+        half = cos.shape[-1] // 2
+        return all(t.dim() == 3 and torch.equal(t[..., :half], t[..., half:]) for t in (cos, sin))
+    except Exception:
+        return False
+
+
+def fused_rotary(original: Any):
+    """``apply_rotary_pos_emb`` of a model as one kernel (``paged.qk_norm_rope``).
+
+    Inputs outside the kernel's -- CPU tensors, gradients, other layouts or
+    dtypes, part of the head rotated -- go to the model's own function.  The
+    kernel computes in float32 and rounds once, where the model's elementwise
+    products round at each step."""
+    from .paged import qk_norm_rope
+
+    @functools.wraps(original)
+    def apply_rotary_pos_emb(q, k, cos, sin, *args, **kwargs):
+        plain = (args or any(v != 1 for n, v in kwargs.items() if n == "unsqueeze_dim")
+                 or any(n != "unsqueeze_dim" for n in kwargs)
+                 or not (q.is_cuda and k.is_cuda and cos.is_cuda and sin.is_cuda)
+                 or q.dim() != 4 or k.dim() != 4 or cos.dim() != 3 or cos.shape != sin.shape
+                 or cos.shape[-1] != q.shape[-1] or cos.shape[1] != q.shape[2] or cos.shape[0] not in (1, q.shape[0])
+                 or q.dtype != k.dtype or q.dtype not in (torch.float32, torch.bfloat16, torch.float16)
+                 or cos.dtype != sin.dtype or cos.dtype not in (q.dtype, torch.float32)
+                 or (q.shape[-1] * q.element_size()) % 16 or q.shape[-1] * q.element_size() > 1024
+                 or (torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, cos, sin))))
+        if plain:
+            return original(q, k, cos, sin, *args, **kwargs)
+        B, _, Q, D = q.shape
+        half = D // 2
+        rows = [t.expand(B, Q, D).reshape(B * Q, D)[:, :half] for t in (cos, sin)]
+        return qk_norm_rope(q, k, rows[0], rows[1])
+
+    apply_rotary_pos_emb._kiv_original = original
+    return apply_rotary_pos_emb
+
+
 class KIVMiddleware:
     """Installs KIV's retrieval attention into a HuggingFace model."""
 
@@ -127,8 +189,13 @@ class KIVMiddleware:
         self._installed = False
         self._original_impl: str | None = None
         self._kiv_key: str | None = None
+        self._rotary_module: Any = None
 
-    def install(self) -> None:
+    def install(self, *, fused_rotary: bool = False) -> None:
+        """Route the model's global layers through KIV.  ``fused_rotary``: also
+        turn queries and keys by one kernel in place of the model's elementwise
+        rotation, for models whose rotation it is (half-split pairs); it stands
+        in the model's module, for every model of that family, until ``uninstall()``."""
         if self._installed:
             logger.warning("KIV middleware already installed.")
             return
@@ -149,6 +216,8 @@ class KIVMiddleware:
             ALL_MASK_ATTENTION_FUNCTIONS._global_mapping[self._kiv_key] = (
                 ALL_MASK_ATTENTION_FUNCTIONS[self._original_impl])
         self._set_attn_impl(self._kiv_key)
+        if fused_rotary:
+            self._fuse_rotary()
         self._installed = True
         logger.info("KIV middleware installed: %d global layers (%d independent, %d shared), "
                     "attn=%s, hot=%d, top_p=%d", len(self.topology.global_layer_indices),
@@ -160,6 +229,11 @@ class KIVMiddleware:
             return
         if self._original_impl is not None:
             self._set_attn_impl(self._original_impl)
+        if self._rotary_module is not None:
+            fn = getattr(self._rotary_module, "apply_rotary_pos_emb", None)
+            if hasattr(fn, "_kiv_original"):
+                self._rotary_module.apply_rotary_pos_emb = fn._kiv_original
+            self._rotary_module = None
         if self._kiv_key is not None:
             if self._kiv_key in ALL_ATTENTION_FUNCTIONS:
                 del ALL_ATTENTION_FUNCTIONS[self._kiv_key]
@@ -247,6 +321,21 @@ class KIVMiddleware:
         if not self._installed:
             raise RuntimeError("Call install() before chunked_retrieval_prefill().")
         return chunked_reuse_prefill(self.model, input_ids, cache, chunk_size=chunk_size)
+
+    def _fuse_rotary(self) -> None:
+        attn = self._text_model.layers[self.topology.global_layer_indices[0]].self_attn
+        module = sys.modules.get(type(attn).__module__)
+        fn = getattr(module, "apply_rotary_pos_emb", None)
+        rotary = getattr(self._text_model, "rotary_emb", None)
+        device = next(self.model.parameters()).device
+        if fn is None or rotary is None or not _turns_half_split(getattr(fn, "_kiv_original", fn), self.topology.head_dim) \
+                or not _repeats_halves(rotary, device):
+            logger.warning("fused_rotary: %s does not rotate half-split pairs through apply_rotary_pos_emb; left as it is",
+                           type(attn).__name__)
+            return
+        if not hasattr(fn, "_kiv_original"):
+            module.apply_rotary_pos_emb = fused_rotary(fn)
+            self._rotary_module = module
 
     def _resolve_attn_impl(self) -> str:
         cfg = self.model.config

@@ -113,3 +113,122 @@ def paged_attend(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
     ops.call(ops.kiv().paged_attend, q, k_pages, v_pages, block_table, seq_lens, q_starts, scaling, causal, window, softcap,
              max_query_len, out, lse, errors)
     return (out, lse) if return_lse else out
+
+
+class PagedKVCache:
+    """Pages of a model's KV layers for a batch of sequences of unequal lengths.
+
+    The pages of a layer are ``k[layer]``, ``v[layer]`` ``[num_pages, Hkv,
+    page_size, D]``; all layers share one block table.  A serving step:
+
+        cache.step([(seq, new_tokens), ...])        # reserves pages, uploads table and lengths
+        for layer in ...:
+            cache.append(layer, k, v, cos=..., sin=...)
+            out = cache.attend(layer, q, scaling)   # packed rows, in the step's order
+
+    ``step`` is host work (it raises before it changes anything when the pages
+    run out); ``append`` and ``attend`` read its device arrays, which stay where
+    they are, so a captured ``append`` / ``attend`` serves later steps of the
+    same batch size and token count.  ``errors`` collects the kernels' bits.
+    """
+
+    def __init__(self, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int, *, layers: int = 1,
+                 dtype: torch.dtype = torch.bfloat16, device: torch.device | str = "cuda", max_batch: int = 64,
+                 max_pages_per_seq: int | None = None) -> None:
+        if min(num_pages, page_size, num_kv_heads, head_dim, layers, max_batch) < 1:
+            raise ValueError("PagedKVCache sizes must be positive")
+        device = torch.device(device)
+        if device.type != "cuda":
+            raise nat.KIVNativeError(f"PagedKVCache runs on CUDA devices only (got {device}); the B200 kernels are the "
+                                     "only implementation")
+        nat.dtype_code(dtype)
+        self.page_size, self.num_pages, self.max_batch = page_size, num_pages, max_batch
+        width = min(num_pages, max_pages_per_seq or num_pages)
+        # zeros: a stale row never reaches a result, whatever it holds, but NaN in a dump would mislead
+        self.k = torch.zeros(layers, num_pages, num_kv_heads, page_size, head_dim, dtype=dtype, device=device)
+        self.v = torch.zeros_like(self.k)
+        self.device = self.k.device
+        self._table = torch.full((max_batch, width), -1, dtype=torch.int32, device=device)
+        self._lens = torch.zeros(max_batch, dtype=torch.int32, device=device)
+        self._starts = torch.zeros(max_batch + 1, dtype=torch.int32, device=device)
+        self.errors = torch.zeros(1, dtype=torch.int64, device=device)
+        self._rows = torch.full((max_batch, width), -1, dtype=torch.int32)     # host copy of the table
+        self._free = list(range(num_pages - 1, -1, -1))
+        self._pages: dict = {}
+        self._length: dict = {}
+        self._batch = self._tokens = self._most = 0
+
+    # ------------------------------------------------------------------ host
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def length(self, seq) -> int:
+        """Tokens of a sequence, those of the current step included (0: unknown)."""
+        return self._length.get(seq, 0)
+
+    def step(self, new: list[tuple]) -> int:
+        """Begin a step: ``new`` lists ``(sequence, new tokens)`` in the order of the packed rows; unknown sequences
+        start empty.  Reserves their pages and uploads table, lengths and row starts.  Returns the number of rows."""
+        if len(new) > self.max_batch:
+            raise ValueError(f"{len(new)} sequences exceed max_batch {self.max_batch}")
+        if len({s for s, _ in new}) != len(new):
+            raise ValueError("a sequence appears twice in one step")
+        need = {}
+        for seq, n in new:
+            if n < 0:
+                raise ValueError("negative token count")
+            pages = -(-(self.length(seq) + n) // self.page_size)
+            if pages > self._table.shape[1]:
+                raise nat.KIVNativeError(f"sequence {seq!r} needs {pages} pages, a sequence holds at most {self._table.shape[1]}")
+            need[seq] = pages - len(self._pages.get(seq, ()))
+        if sum(need.values()) > len(self._free):
+            raise nat.KIVNativeError(f"out of pages: the step needs {sum(need.values())}, {len(self._free)} are free")
+        starts, lens = [0], []
+        rows = self._rows[:len(new)].clone()
+        for i, (seq, n) in enumerate(new):
+            held = self._pages.setdefault(seq, [])
+            held.extend(self._free.pop() for _ in range(need[seq]))
+            self._length[seq] = self.length(seq) + n
+            lens.append(self._length[seq])
+            starts.append(starts[-1] + n)
+            rows[i, :len(held)] = torch.tensor(held, dtype=torch.int32)
+            rows[i, len(held):] = -1
+        changed = (rows != self._rows[:len(new)]).any(1).nonzero().flatten().tolist()
+        self._rows[:len(new)] = rows
+        if changed:
+            lo, hi = changed[0], changed[-1] + 1
+            self._upload(self._table[lo:hi], rows[lo:hi])
+        self._upload(self._lens[:len(new)], torch.tensor(lens, dtype=torch.int32))
+        self._upload(self._starts[:len(new) + 1], torch.tensor(starts, dtype=torch.int32))
+        self._batch, self._tokens, self._most = len(new), starts[-1], max([n for _, n in new], default=0)
+        return self._tokens
+
+    def _upload(self, dst: torch.Tensor, src: torch.Tensor) -> None:
+        if src.numel():
+            dst.copy_(src.pin_memory(), non_blocking=True)     # a fresh pinned buffer: the allocator keeps it until the copy is done
+
+    def free(self, seq) -> None:
+        """Give a sequence's pages back (a step that is still running may read them: free after it)."""
+        self._free.extend(reversed(self._pages.pop(seq, [])))
+        self._length.pop(seq, None)
+
+    # ---------------------------------------------------------------- device
+    def arrays(self) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """``(block_table, seq_lens, q_starts)`` of the current step."""
+        return self._table[:self._batch], self._lens[:self._batch], self._starts[:self._batch + 1]
+
+    def _check(self, rows: torch.Tensor) -> None:
+        if rows.shape[0] < self._tokens:
+            raise nat.KIVNativeError(f"the step has {self._tokens} rows, got {rows.shape[0]}")
+
+    def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, **turn) -> None:
+        """Write the step's new rows of a layer (``paged_append``; ``turn``: its keyword arguments)."""
+        self._check(k)
+        paged_append(k, v, self.k[layer], self.v[layer], *self.arrays(), errors=self.errors, **turn)
+
+    def attend(self, layer: int, q: torch.Tensor, scaling: float, **kw):
+        """Attention of the step's new tokens over a layer's pages (``paged_attend``)."""
+        self._check(q)
+        return paged_attend(q, self.k[layer], self.v[layer], *self.arrays(), scaling, max_query_len=self._most,
+                            errors=self.errors, **kw)

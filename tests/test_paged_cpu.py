@@ -177,3 +177,55 @@ def test_rotary_tables_are_exact_at_far_positions():
     far = torch.tensor([(1 << 20) - 1.0], dtype=torch.float64)
     assert cos.dtype == torch.float32 and cos.shape == (1 << 20, 2)
     assert torch.equal(cos[-1], (2 * torch.cos(far * inv)).float()) and torch.equal(sin[-1], (2 * torch.sin(far * inv)).float())
+
+
+def test_paged_cache_needs_a_gpu():
+    from kiv_b200 import PagedKVCache
+    with pytest.raises(nat.KIVNativeError, match="CUDA devices only"):
+        PagedKVCache(4, 16, 1, 64, device="cpu")
+    with pytest.raises(ValueError):
+        PagedKVCache(0, 16, 1, 64, device="cpu")
+
+
+def test_fused_rotation_stands_in_and_leaves_again():
+    """On the CPU the model's own function answers, to the bit; another convention is left alone."""
+    import sys
+    from transformers import LlamaConfig, LlamaForCausalLM
+    from kiv_b200 import KIVConfig, KIVMiddleware
+    from kiv_b200 import middleware as mid
+
+    torch.manual_seed(0)
+    model = LlamaForCausalLM(LlamaConfig(vocab_size=64, hidden_size=64, intermediate_size=64, num_hidden_layers=1,
+                                         num_attention_heads=2, num_key_value_heads=1, head_dim=32,
+                                         attn_implementation="eager")).eval()
+    module = sys.modules[type(model.model.layers[0].self_attn).__module__]
+    before = module.apply_rotary_pos_emb
+    ids = torch.arange(10)[None]
+    want = model(input_ids=ids, use_cache=False).logits
+    mw = KIVMiddleware(model, KIVConfig())
+    mw.install()
+    assert module.apply_rotary_pos_emb is before            # off by default
+    mw.uninstall()
+    mw.install(fused_rotary=True)
+    assert module.apply_rotary_pos_emb is not before
+    other = KIVMiddleware(model, KIVConfig())
+    other._text_model, other.topology = mw._text_model, mw.topology
+    other._fuse_rotary()                                    # already there: neither stacked nor taken out by another
+    assert module.apply_rotary_pos_emb._kiv_original is before and other._rotary_module is None
+    assert torch.equal(model(input_ids=ids, use_cache=False).logits, want)
+    mw.uninstall()
+    assert module.apply_rotary_pos_emb is before
+
+    def adjacent(q, k, cos, sin, unsqueeze_dim=1):
+        c, s = cos.unsqueeze(unsqueeze_dim), sin.unsqueeze(unsqueeze_dim)
+        turn = lambda x: x * c + torch.stack([-x[..., 1::2], x[..., ::2]], -1).flatten(-2) * s
+        return turn(q), turn(k)
+
+    assert mid._turns_half_split(before, 32) and not mid._turns_half_split(adjacent, 32)
+    module.apply_rotary_pos_emb = adjacent
+    try:
+        mw.install(fused_rotary=True)
+        assert module.apply_rotary_pos_emb is adjacent
+        mw.uninstall()
+    finally:
+        module.apply_rotary_pos_emb = before
