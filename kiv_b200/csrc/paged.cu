@@ -83,14 +83,13 @@ __global__ void __launch_bounds__(CC_THREADS) paged_cc_kernel(const __grid_const
   constexpr int RPT = R / 16;          // rows per thread
   constexpr int DC = (DM + 63) / 64;   // 4-element slices of an output row per thread
   extern __shared__ float4 cc_dyn[];
-  __shared__ int64_t sm[40];
   __shared__ int64_t s_ko[CC_KEYS], s_vo[CC_KEYS];
   const int D = p.pc.head_dim, nv = D / V, ld = D + 4;
   float *sq = reinterpret_cast<float *>(cc_dyn);
   float *sk = sq + R * ld, *sv = sk + CC_KEYS * ld, *sp = sv + CC_KEYS * ld;
   const int tr = threadIdx.x / 16, tc = threadIdx.x % 16;
   griddep_wait();
-  PagedSpot at = paged_locate<CC_THREADS>(p, sm);
+  PagedSpot at = paged_locate(p);              // every warp for itself
   if (threadIdx.x == 0) p.cut[blockIdx.x].b = -1;
   while (at.it.s.b >= 0 && at.unit < at.end) {
     const PagedSegment g = paged_segment(p, at);
@@ -265,17 +264,15 @@ __global__ void __launch_bounds__(CC_THREADS) paged_cc_kernel(const __grid_const
         }
       }
     }
-    at.unit += g.t1 - g.t0;
-    if (g.tail) break;
-    paged_next(p, at);
+    paged_advance(p, at, g);
   }
 }
 
 // ---------------------------------------------------------------------------
 // Join of the items that blocks share.  Block (c, y) takes the item that block
 // c of the attention kernel began and did not finish; a warp takes a row's
-// slice of 128 columns: the parts' maxima first, then their scaled sum, in
-// block order.
+// slice of 128 columns: the parts' maxima and sums by lane, then the scaled sum
+// of the parts in block order.
 // ---------------------------------------------------------------------------
 constexpr int CB_WARPS = 8;
 
@@ -286,36 +283,62 @@ __global__ void __launch_bounds__(CB_WARPS * 32) paged_combine_kernel(const __gr
   if (cut.b < 0) return;
   const int D = p.pc.head_dim, lane = threadIdx.x & 31;
   const int slices = (D + 127) / 128;
-  const PagedItems it = paged_items(p, cut.b);
+  PagedItems it;
+  it.s.b = cut.b;
+  it.s.q0 = cut.q0;
+  it.s.n = cut.n;
   const int warp = (blockIdx.y * CB_WARPS + (threadIdx.x >> 5)), nwarps = gridDim.y * CB_WARPS;
-  // parts: slot 2c + 1, then slot 2c' of each later block c' whose stretch
-  // begins inside the item (c' N / G < end)
-  const int c0 = blockIdx.x;
-  const int last = (int)((cut.end * cut.blocks - 1) / cut.total);
+  // parts: slot 2c + 1, then slot 2c' of the later blocks up to the last
+  const int c0 = blockIdx.x, last = cut.last;
+  const int64_t stride = 2 * (int64_t)p.rows * partial_stride(D);
   for (int x = warp; x < p.tpt * p.grp * slices; x += nwarps) {
     const int r = x / slices, col = (x % slices) * 128 + 4 * lane;
     int i, head;
     if (!paged_row(p, it, cut.hp, cut.rt, r, i, head)) continue;
-    float mx = -INFINITY;
-    for (int c = c0 + lane; c <= last; c += 32) {
-      mx = fmaxf(mx, paged_part(p, 2 * (int64_t)c + (c == c0), r)[D]);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(KIV_FULL_MASK, mx, o));
-    const float ms = mx == -INFINITY ? 0.f : mx;
-    float l = 0.f;
+    // lane k holds maximum and sum of part k of 32 at a time; the parts' values
+    // are asked for eight at a time, the first of them before the maxima
+    float mx = -INFINITY, l = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int c = c0; c <= last; ++c) {
-      const float *src = paged_part(p, 2 * (int64_t)c + (c == c0), r);
-      const float w = ex2((src[D] - ms) * 1.44269504f);
-      l = fmaf(src[D + 1], w, l);
-      if (col < D) {
-        const float4 v = *reinterpret_cast<const float4 *>(src + col);
-        acc.x = fmaf(v.x, w, acc.x);
-        acc.y = fmaf(v.y, w, acc.y);
-        acc.z = fmaf(v.z, w, acc.z);
-        acc.w = fmaf(v.w, w, acc.w);
+    for (int c1 = c0; c1 <= last; c1 += 32) {
+      const int n = min(32, last - c1 + 1);
+      const float *src = paged_part(p, 2 * (int64_t)c1, r);
+      const int64_t shift = c1 == c0 ? stride / 2 : 0;           // of part 0
+      const float *mine = src + lane * stride + (lane == 0 ? shift : 0);
+      const float2 ml = lane < n ? *reinterpret_cast<const float2 *>(mine + D) : make_float2(-INFINITY, 0.f);
+      float4 v[8];
+      auto ask = [&](int k0) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          v[k] = k0 + k < n && col < D ? *reinterpret_cast<const float4 *>(src + (k0 + k) * stride + (k0 + k == 0 ? shift : 0) + col)
+                                       : make_float4(0.f, 0.f, 0.f, 0.f);
+      };
+      ask(0);
+      float top = ml.x;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(KIV_FULL_MASK, top, o));
+      top = fmaxf(top, mx);
+      const float ms = top == -INFINITY ? 0.f : top, keep = ex2((mx - ms) * 1.44269504f);
+      const float w = ex2((ml.x - ms) * 1.44269504f);
+      float sum = ml.y * w;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(KIV_FULL_MASK, sum, o);
+      l = l * keep + sum;
+      mx = top;
+      acc.x *= keep;
+      acc.y *= keep;
+      acc.z *= keep;
+      acc.w *= keep;
+#pragma unroll 1
+      for (int k0 = 0; k0 < n; k0 += 8) {
+        if (k0 > 0) ask(k0);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float f = __shfl_sync(KIV_FULL_MASK, w, k0 + k);
+          acc.x = fmaf(v[k].x, f, acc.x);
+          acc.y = fmaf(v[k].y, f, acc.y);
+          acc.z = fmaf(v[k].z, f, acc.z);
+          acc.w = fmaf(v[k].w, f, acc.w);
+        }
       }
     }
     const float inv = l > 0.f ? 1.f / l : 0.f;
@@ -333,7 +356,8 @@ __global__ void __launch_bounds__(CB_WARPS * 32) paged_combine_kernel(const __gr
 kiv_status launch_paged_combine(const PagedPlan &p, int blocks, cudaStream_t s) {
   if (blocks < 2) return KIV_OK;
   const int slices = (int)ceil_div(p.pc.head_dim, 128);
-  const int y = (int)std::min<int64_t>(ceil_div((int64_t)p.tpt * p.grp * slices, CB_WARPS), 32);
+  const int64_t rows = std::min<int64_t>(p.tpt, p.pc.num_tokens) * p.grp;    // of an item at most
+  const int y = (int)std::min<int64_t>(ceil_div(rows * slices, CB_WARPS), 32);
   const dim3 grid((unsigned)blocks, (unsigned)y), block(CB_WARPS * 32);
   cudaError_t e;
   if (p.pc.dtype == KIV_DTYPE_F32) e = launch_pdl(paged_combine_kernel<float>, grid, block, 0, s, 1, p);
@@ -351,8 +375,9 @@ static PagedPlan make_plan(const kiv_paged *pc, const kiv_paged_query *q, int ro
   const int per = q->num_query_heads / pc->num_kv_heads;
   p.hs = (int)ceil_div(per, rows);
   p.grp = (int)ceil_div(per, p.hs);
-  p.tpt = rows / p.grp;
+  p.tpt = p.tps = rows / p.grp;
   p.kt = kt;
+  p.kt_log2 = kt == 64 ? 6 : 7;
   p.rows = rows;
   return p;
 }
@@ -368,8 +393,8 @@ struct PagedCall {
 };
 
 // The kernel of a call and its tiling.  tcgen05 wherever TMA can bring the
-// pages (paged_tc.cu): for single tokens too, 210 us against 250 (64 x 16 k
-// keys of 32/8 x 128) and 62 against 84 (8/1 x 256) by the split kernel, which
+// pages (paged_tc.cu): for single tokens too, 209 us against 249 (16 sequences of
+// 16 k keys, 32/8 x 128) and 62 against 84 (8/1 x 256) by the split kernel, which
 // keeps the pages of odd sizes and strides, the head dimensions 80 and 192 and
 // heads in groups above 128; CUDA cores for fp32 and what is left.  The lengths
 // are on the device, so the row tiles of the latter two go by what the host

@@ -55,14 +55,16 @@ __device__ __forceinline__ int paged_find_seq(const kiv_paged &pc, int64_t tok) 
 // ---------------------------------------------------------------------------
 // Division of the work.
 //
-// An item is one row tile of one sequence and one key head: `tpt` new tokens
-// with all the query heads of the key head (cut into `hs` parts where there
-// are more of them than a tile has rows).  Its work is the tiles of `kt` keys
-// that some row of it sees.  The items of the batch, in the order (sequence,
-// head part, row tile), make one line of tiles, and block c of G takes the
-// tiles [c N / G, (c + 1) N / G) of it (G at most N: the other blocks leave):
-// every block streams the same number of key tiles (within one), whatever the
-// lengths.  An item inside one block
+// An item is one or two row tiles of one sequence and one key head: `tpt` new
+// tokens with all the query heads of the key head (cut into `hs` parts where
+// there are more of them than a tile has rows).  Its work is the tiles of `kt`
+// keys that some row of it sees, each counted once per row tile: two row tiles
+// take about twice as long over a key tile as one.  The items of the batch, in
+// the order (sequence, head part, item), make one line of N units, and block c
+// of G takes the key tiles that begin in its stretch [c N / G, (c + 1) N / G)
+// (G at most N, or N / 2 with two row tiles, so that no stretch inside an item
+// is empty: the other blocks leave): every block does the same work (within a
+// tile), whatever the lengths.  An item inside one block
 // is finished there; one that blocks share leaves its parts (running maximum,
 // sum, unscaled output) in the workspace, at most two per block -- slot 2c for
 // an item that began in an earlier block, slot 2c + 1 for one that began in
@@ -70,15 +72,17 @@ __device__ __forceinline__ int paged_find_seq(const kiv_paged &pc, int64_t tok) 
 // so the result does not depend on timing.
 //
 // N, and where a block begins, follow from the lengths alone; each block works
-// them out for itself at its start (one read of the lengths, one block scan).
+// them out for itself at its start (one read of the lengths, one warp scan).
 // ---------------------------------------------------------------------------
 struct PagedPlan {
   kiv_paged pc;
   kiv_paged_query q;
   int grp;       // query heads per head part
   int hs;        // head parts per key head
-  int tpt;       // tokens per row tile
-  int kt;        // keys per key tile
+  int tpt;       // tokens per item
+  int tps;       // tokens per row tile: an item has one (tps = tpt) or two (tpt = 2 tps)
+  int kt;        // keys per key tile: a power of two
+  int kt_log2;
   int rows;      // rows per part in the workspace: tpt * grp <= rows
   float *part;   // [2 * G][rows][D + 2 (rounded to 4)]
   struct PagedCut *cut;     // [G]
@@ -86,9 +90,9 @@ struct PagedPlan {
 
 // What block c says about the item it began and did not finish (b = -1: none)
 struct PagedCut {
-  int32_t b, hp, rt, pad;
-  int64_t end, total;       // the place past the item's last tile; N
-  int64_t blocks;           // blocks that took part
+  int32_t b, hp, rt, n;     // n: new tokens of the sequence
+  int64_t q0;               // packed row of its first
+  int32_t last, pad;        // the last block that holds a part
 };
 
 // sum over i < n of floor((a i + b) / m), a and b not negative: lattice points
@@ -134,7 +138,7 @@ struct PagedItems {      // the items of one sequence
 __device__ __forceinline__ PagedItems paged_items(const PagedPlan &p, int b) {
   PagedItems it;
   it.s = paged_seq(p.pc, b);
-  it.nrt = (it.s.n + p.tpt - 1) / p.tpt;
+  it.nrt = (uint32_t)(it.s.n + p.tpt - 1) / (uint32_t)p.tpt;
   it.base = p.q.causal ? it.s.len - it.s.n : it.s.len;
   return it;
 }
@@ -158,7 +162,7 @@ __host__ __device__ inline void paged_range(const PagedPlan &p, const PagedItems
 __host__ __device__ inline int paged_tiles(const PagedPlan &p, const PagedItems &it, int rt) {
   int lo, hi;
   paged_range(p, it, rt, lo, hi);
-  return (hi + p.kt - 1) / p.kt - lo / p.kt;
+  return ((hi + p.kt - 1) >> p.kt_log2) - (lo >> p.kt_log2);
 }
 
 // tiles of the row tiles [0, x) of one head part
@@ -184,91 +188,93 @@ __host__ __device__ inline int64_t paged_prefix(const PagedPlan &p, const PagedI
   return r;
 }
 
-struct PagedSpot {       // a place on the line of tiles
+// a / b, b > 0: mostly small numbers, and a 64-bit division takes four times a 32-bit one
+__host__ __device__ inline int64_t paged_div(int64_t a, int64_t b) {
+  return ((uint64_t)(a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
+
+// Row tiles of item rt: 1 or 2; its work
+__host__ __device__ inline int paged_weight(const PagedPlan &p, const PagedItems &it, int rt) {
+  return p.tps < p.tpt && it.s.n - rt * p.tpt > p.tps ? 2 : 1;
+}
+__host__ __device__ inline int64_t paged_units(const PagedPlan &p, const PagedItems &it, int rt) {
+  return (int64_t)paged_tiles(p, it, rt) * paged_weight(p, it, rt);
+}
+// work of the items [0, x) of one head part: only the last may have one row tile of two
+__host__ __device__ inline int64_t paged_line(const PagedPlan &p, const PagedItems &it, int x) {
+  const int64_t r = paged_prefix(p, it, x);
+  if (p.tps == p.tpt || x == 0) return r;
+  return 2 * r - (x == it.nrt && paged_weight(p, it, x - 1) == 1 ? paged_tiles(p, it, x - 1) : 0);
+}
+
+struct PagedSpot {       // a place on the line
   PagedItems it;
   int hp;                // key head * hs + head part
   int rt;
-  int64_t off;           // tiles into the item
+  int64_t off;           // units into the item
   int64_t total;         // N
   int64_t blocks;        // G
   int64_t unit;          // the place itself
   int64_t end;           // where the block's stretch ends
 };
 
-// The stretch of this block (blockIdx.x), found by the whole block.  `sm`:
-// shared, 40 words of 8 bytes.  b = -1 in the result: nothing to do.
-template <int NT>
-__device__ __forceinline__ PagedSpot paged_locate(const PagedPlan &p, int64_t *sm) {
-  const int H = p.pc.num_kv_heads * p.hs;
-  const int per = (p.pc.batch + NT - 1) / NT;
-  const int b0 = threadIdx.x * per, b1 = min(b0 + per, p.pc.batch);
+// The stretch of this block (blockIdx.x), found by one whole warp.  b = -1 in
+// the result: nothing to do.
+__device__ __forceinline__ PagedSpot paged_locate(const PagedPlan &p) {
+  const int H = p.pc.num_kv_heads * p.hs, lane = threadIdx.x & 31;
+  const int per = (p.pc.batch + 31) / 32;
+  const int b0 = lane * per, b1 = min(b0 + per, p.pc.batch);
   int64_t mine = 0;
-  PagedItems first;
   for (int b = b0; b < b1; ++b) {
     const PagedItems it = paged_items(p, b);
-    if (b == b0) first = it;
-    if (it.nrt > 0) mine += H * paged_prefix(p, it, it.nrt);
+    if (it.nrt > 0) mine += H * paged_line(p, it, it.nrt);
   }
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int64_t inc = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int64_t y = __shfl_up_sync(KIV_FULL_MASK, inc, o);
     if (lane >= o) inc += y;
   }
-  __syncthreads();
-  if (lane == 31) sm[warp] = inc;
-  if (threadIdx.x == 0) sm[32] = -1;
-  __syncthreads();
-  int64_t before = 0, total = 0;
-  for (int w = 0; w < NT / 32; ++w) {
-    if (w < warp) before += sm[w];
-    total += sm[w];
-  }
-  const int64_t G = min((int64_t)gridDim.x, total), c = blockIdx.x;
-  const int64_t unit = c < G ? c * total / G : total;   // below 2^63: N counts tiles, c blocks
-  int64_t at = unit - (before + inc - mine);
-  if (at >= 0 && at < mine) {
-    for (int b = b0; b < b1; ++b) {
-      const PagedItems it = b == b0 ? first : paged_items(p, b);
-      const int64_t c = it.nrt > 0 ? H * paged_prefix(p, it, it.nrt) : 0;
-      if (at < c) {
-        sm[32] = b;
-        sm[33] = at;
-        break;
-      }
-      at -= c;
-    }
-  }
-  __syncthreads();
+  const int64_t total = __shfl_sync(KIV_FULL_MASK, inc, 31);
+  const int64_t G = min((int64_t)gridDim.x, p.tps < p.tpt ? (total + 1) / 2 : total), c = blockIdx.x;
   PagedSpot r;
   r.total = total;
   r.blocks = G;
-  r.unit = unit;
-  r.end = c < G ? (c + 1) * total / G : total;
+  r.unit = c < G ? paged_div(c * total, G) : total;   // below 2^63: N counts tiles, c blocks
+  r.end = c < G ? paged_div((c + 1) * total, G) : total;
   r.hp = r.rt = 0;
   r.off = 0;
-  const int b = (int)sm[32];
-  if (b < 0) {
-    r.it.s.b = -1;
-    r.it.nrt = 0;
-    return r;
+  r.it.s.b = -1;
+  r.it.nrt = 0;
+  if (c >= G) return r;
+  // the lane whose sequences hold the place, then the sequence among them
+  int64_t at = r.unit - (inc - mine);
+  const int owner = __ffs(__ballot_sync(KIV_FULL_MASK, at >= 0 && at < mine)) - 1;
+  int b = b0;
+  if (lane == owner) {
+    for (; b < b1; ++b) {
+      const PagedItems it = paged_items(p, b);
+      const int64_t n = it.nrt > 0 ? H * paged_line(p, it, it.nrt) : 0;
+      if (at < n) break;
+      at -= n;
+    }
   }
+  b = __shfl_sync(KIV_FULL_MASK, b, owner);
+  int64_t rem = __shfl_sync(KIV_FULL_MASK, at, owner);
   r.it = paged_items(p, b);
-  int64_t rem = sm[33];
-  const int64_t per_head = paged_prefix(p, r.it, r.it.nrt);
-  r.hp = (int)(rem / per_head);
+  const int64_t per_head = paged_line(p, r.it, r.it.nrt);
+  r.hp = (int)paged_div(rem, per_head);
   rem -= (int64_t)r.hp * per_head;
   // largest rt with prefix(rt) <= rem: the lanes try 32 places at a time
   int a = 0, z = r.it.nrt;
   while (z - a > 1) {
     const int stride = (z - a + 31) / 32, x = a + lane * stride;
-    const unsigned under = __ballot_sync(KIV_FULL_MASK, x < z && paged_prefix(p, r.it, x) <= rem);
+    const unsigned under = __ballot_sync(KIV_FULL_MASK, x < z && paged_line(p, r.it, x) <= rem);
     a += (31 - __clz(under)) * stride;           // lane 0 always holds
     z = min(z, a + stride);
   }
   r.rt = a;
-  r.off = rem - paged_prefix(p, r.it, a);
+  r.off = rem - paged_line(p, r.it, a);
   return r;
 }
 
@@ -288,15 +294,15 @@ __device__ __forceinline__ void paged_next(const PagedPlan &p, PagedSpot &s) {
 
 // One segment of a block's stretch [at.unit, at.end): the item's tiles [t0, t1)
 struct PagedSegment {
-  int t0, t1;
+  int t0, t1;            // equal: the stretch ends on the item's first units, without a whole tile
   bool head, tail;       // the item began in an earlier block / goes on in a later one
 };
 
 __device__ __forceinline__ PagedSegment paged_segment(const PagedPlan &p, const PagedSpot &at) {
   PagedSegment g;
-  const int nt = paged_tiles(p, at.it, at.rt);
-  g.t0 = (int)at.off;
-  g.t1 = (int)min((int64_t)nt, at.off + (at.end - at.unit));
+  const int nt = paged_tiles(p, at.it, at.rt), shift = paged_weight(p, at.it, at.rt) - 1;
+  g.t0 = (int)(at.off >> shift);
+  g.t1 = (int)min((int64_t)nt, (at.off + (at.end - at.unit)) >> shift);
   g.head = g.t0 > 0;
   g.tail = g.t1 < nt;
   return g;
@@ -310,11 +316,24 @@ __device__ __forceinline__ void paged_record(const PagedPlan &p, int c, const Pa
     r.b = at.it.s.b;
     r.hp = at.hp;
     r.rt = at.rt;
-    r.end = at.unit - at.off + paged_tiles(p, at.it, at.rt);
-    r.total = at.total;
-    r.blocks = at.blocks;
+    r.n = at.it.s.n;
+    r.q0 = at.it.s.q0;
+    // the block of the item's last tile: the last c' whose stretch begins
+    // (c' N / G) before the item's end
+    const int64_t end = at.unit - at.off + paged_units(p, at.it, at.rt);
+    r.last = (int)((end * at.blocks - 1) / at.total);
   }
   p.cut[c] = r;
+}
+
+// On to the next item of the stretch, or to its end (b = -1)
+__device__ __forceinline__ void paged_advance(const PagedPlan &p, PagedSpot &at, const PagedSegment &g) {
+  if (g.tail) {
+    at.it.s.b = -1;
+    return;
+  }
+  at.unit += paged_units(p, at.it, at.rt) - at.off;
+  paged_next(p, at);
 }
 
 __device__ __forceinline__ void paged_check_lens(const kiv_paged &pc, const PagedSeq &s) {
@@ -328,7 +347,7 @@ __device__ __forceinline__ float *paged_part(const PagedPlan &p, int64_t slot, i
 
 // Row r of an item's tile: token (in the sequence) and query head, or false
 __device__ __forceinline__ bool paged_row(const PagedPlan &p, const PagedItems &it, int hp, int rt, int r, int &i, int &head) {
-  const int ti = r / p.grp, g = r - ti * p.grp;
+  const int ti = (uint32_t)r / (uint32_t)p.grp, g = r - ti * p.grp;
   i = rt * p.tpt + ti;
   const int per = p.q.num_query_heads / p.pc.num_kv_heads;
   const int gi = (hp % p.hs) * p.grp + g;

@@ -1,16 +1,15 @@
-// Paged attention of few query rows per key head (decode, drafted tokens):
-// split over the keys, 16-bit rows, warp-level tensor-core MMAs.
+// Paged attention of 16-bit rows with warp-level tensor-core MMAs, for what the
+// tcgen05 kernels do not take (plan_call in paged.cu): pages whose size is no
+// multiple of 8, head dimensions 80 and 192, large groups, expanded strides.
 //
-// Bound by memory: with r query rows a key head's K and V rows carry 2 r FLOP
-// per byte, so up to about a hundred rows HBM is the limit and the kernel has
-// to keep it busy.  A block streams tiles of 64 keys through a ring of shared
+// Made for few query rows: with r of them a key head's K and V rows carry 2 r
+// FLOP per byte, and HBM is the limit.  A block streams tiles of 64 keys through a ring of shared
 // memory, one bulk copy per row (any page size, any row stride): each of the
 // 128 threads brings one K or V row of every tile, whose page number it read a
 // step before.  With 16-byte cp.async instead, the address arithmetic alone
-// was a third of the instructions and the kernel issue-bound at 2.4 TB/s.  The
-// blocks share the batch's tiles evenly (paged.cuh).  tcgen05
-// is of no use here: its tile has 128 rows, and the m16n8k16 MMAs take a
-// fraction of the time a tile needs to arrive.
+// was a third of the instructions and the kernel issue-bound at 2.4 TB/s, where
+// this reaches 4.9 (64 sequences of up to 32 k keys, 32/8 x 128).  The blocks
+// share the batch's tiles evenly (paged.cuh).
 //
 // WM x WN = 4 warps: WM groups of 16 query rows, WN groups of keys.  Each warp
 // runs its own softmax over its keys (maximum, sum and output in registers);
@@ -101,7 +100,6 @@ __global__ void __launch_bounds__(MM_THREADS, MmaShape<D, 16 * WM>::BLOCKS) page
   constexpr bool EXACT = WM == 1;
   constexpr bool QREG = D <= 128;              // query fragments stay in registers
   extern __shared__ __align__(128) uint8_t mm_dyn[];
-  __shared__ int64_t sm[40];
   __shared__ uint64_t full[STAGES];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int wm = warp % WM, wn = warp / WM;
@@ -112,7 +110,7 @@ __global__ void __launch_bounds__(MM_THREADS, MmaShape<D, 16 * WM>::BLOCKS) page
     mbar_fence_init();
   }
   griddep_wait();
-  PagedSpot at = paged_locate<MM_THREADS>(p, sm);
+  PagedSpot at = paged_locate(p);              // every warp for itself
   if (threadIdx.x == 0) p.cut[blockIdx.x].b = -1;
   const float scale = p.q.scaling;
   // this thread's row of every tile
@@ -363,9 +361,7 @@ __global__ void __launch_bounds__(MM_THREADS, MmaShape<D, 16 * WM>::BLOCKS) page
         }
       }
     }
-    at.unit += ntile;
-    if (sg.tail) break;
-    paged_next(p, at);
+    paged_advance(p, at, sg);
   }
   if (!ok) paged_error(p.pc.errors, KIV_ERRBIT_WAIT_TIMEOUT);
 }

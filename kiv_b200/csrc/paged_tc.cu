@@ -1,4 +1,5 @@
-// Paged attention of chunks (many query rows per key head) on tcgen05.
+// Paged attention on tcgen05, head dimensions 64, 96 and 128: chunks of new
+// tokens (bound by the tensor cores) and single ones (bound by memory).
 //
 //   S = Q K^T and O += P V as 128 x 128 x D and 128 x D x 128 products with
 //   fp32 accumulators in TMEM; the softmax in between is one pass with the
@@ -16,12 +17,17 @@
 // softmax -> product exposed: there both take the same rows, one over the even
 // key tiles and one over the odd ones, and join at the end ("twins").  So the
 // same kernel serves decode, bound by memory: warps without rows only keep the
-// beat, and the tensor cores' empty rows cost nothing that is missed (CUDA-core
-// free m16n8k16 products took TWIN_CMP).
+// beat, and the tensor cores' empty rows cost nothing that is missed.  Measured
+// over 16 sequences of 16 k keys, one token each: 32/8 x 128 209 us (5.0 TB/s)
+// and 32/4 x 64 76 us, against 249 and 100 us for m16n8k16 products split over
+// the keys (paged_mma.cu); without twins 32/4 x 64 takes 97 us.
 // While one row tile's softmax runs, the tensor cores work on the other's
 // products, so both are kept busy: per tile pair the tensor cores need 4 x 512
 // cycles (D = 128) and the 2 x 16384 exponentials 2048 cycles of the special
-// function units.
+// function units.  Measured: 4096 tokens over 36864 keys, 32/8 x 128: 2.2-2.4 ms,
+// 1.0-1.06 PFLOP/s at the power limit (1.3-1.4 GHz); with the softmax taken out
+// the products alone take 1.6 ms.  One warp issuing both row tiles' products
+// took 3950 cycles per tile pair where this takes 3240.
 //
 // P (16-bit) overwrites S in TMEM and is the A operand from there; V is read
 // as an MN-major B operand straight from its row-major tile.  The output in
@@ -59,7 +65,6 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
   constexpr int SLOTS = S::SLOTS;
   extern __shared__ uint8_t pt_dyn[];
   __shared__ uint64_t q_full, q_empty, kv_full[SLOTS], kv_empty[SLOTS], s_full[2], p_full[2], p_tail[2], o_full[2];
-  __shared__ int64_t sm[40];
   __shared__ uint32_t s_tmem;
   __shared__ PtSeg seg[2];
   __shared__ float s_ml[2][PT_ROWS];           // of the second of two twins
@@ -100,8 +105,6 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
   tc::fence_after_sync();
   const uint32_t tmem = s_tmem;
   griddep_wait();
-  PagedSpot at = paged_locate<PT_THREADS>(p, sm);
-  if (threadIdx.x == 0) p.cut[blockIdx.x].b = -1;
   bool ok = true;
   const int rows = g.tps * p.grp;              // of a row tile
   if (warp >= 8) {
@@ -112,44 +115,56 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
     // is 16 copies, and one warp issued them at 5.0 TB/s, no faster.
     const int me = warp == 8 ? 0 : 1;
     const bool leader = elect_one();
+    PagedSpot at = paged_locate(p);
     uint32_t n = 0, items = 0;
+    const int nbox = PT_KEYS / g.br;
+    if (me == 0 && lane == 0) p.cut[blockIdx.x].b = -1;
     for (;; ++items) {
-      const bool live = at.it.s.b >= 0 && at.unit < at.end;
       PtSeg sg = {};
       PagedSegment cut = {};
       int kvh = 0;
-      if (live) sg = pt_segment(p, at, g.tps, cut, kvh);
-      if (me == 0 && items > 0 && ok && !mbar_wait_bounded(&q_empty, (items - 1) & 1)) ok = false;
-      if (me == 0 && lane == 0) {
-        seg[items & 1] = sg;
-        if (!live) {
-          mbar_arrive(&q_full);
-        } else {
-          if (!cut.head) paged_check_lens(p.pc, at.it.s);
-          if (cut.tail) paged_record(p, blockIdx.x, at, cut);
-          mbar_arrive_tx(&q_full, (uint32_t)sg.nsub * rows * D * 2);
-          for (int i = 0; i < sg.nsub; ++i)
-            for (int c = 0; c < S::NB; ++c)
-              tc::tma_load_3d(qmem + i * S::TILE + c * (PT_ROWS * S::BOXB), &qmap, c * S::BOX, sg.head0,
-                              (int32_t)(sg.q0 + i * g.tps), &q_full);
-        }
-      }
-      if (!live) break;
-      __syncwarp();
+      if (at.it.s.b >= 0 && at.unit < at.end) sg = pt_segment(p, at, g.tps, cut, kvh);
+      const int ntile = sg.ntile;              // 0: done
       // lane l brings rows [l br, (l + 1) br) of every tile
-      const int nbox = PT_KEYS / g.br;
-      const int32_t *table = p.pc.block_table + at.it.s.b * p.pc.table_stride;
+      const int32_t *table = p.pc.block_table + (ntile > 0 ? at.it.s.b : 0) * p.pc.table_stride;
       auto lookup = [&](int t, int32_t &page, int32_t &row) {
         page = -1;
         row = 0;
-        if (t < sg.ntile && lane < nbox) pt_lookup(p, table, sg, sg.j00 + (int64_t)t * PT_KEYS + lane * g.br, g.br, page, row);
+        if (t < ntile && lane < nbox) pt_lookup(p, table, sg, sg.j00 + (int64_t)t * PT_KEYS + lane * g.br, g.br, page, row);
       };
       int32_t page, row;
       lookup(0, page, row);
-      for (int t = 0; t < sg.ntile; ++t) {
+      // The queries and `seg` replace the previous item's when those are used
+      // up; until then this item's first keys and values can come.
+      bool told = me != 0;
+      auto tell = [&](bool must) {
+        if (told) return;
+        if (items > 0 && !must && !__shfl_sync(KIV_FULL_MASK, (int)mbar_test(&q_empty, (items - 1) & 1), 0)) return;
+        if (items > 0 && ok && !mbar_wait_bounded(&q_empty, (items - 1) & 1)) ok = false;
+        if (lane == 0) {
+          seg[items & 1] = sg;
+          if (ntile == 0) {
+            mbar_arrive(&q_full);
+          } else {
+            mbar_arrive_tx(&q_full, (uint32_t)sg.nsub * rows * D * 2);
+            for (int i = 0; i < sg.nsub; ++i)
+              for (int c = 0; c < S::NB; ++c)
+                tc::tma_load_3d(qmem + i * S::TILE + c * (PT_ROWS * S::BOXB), &qmap, c * S::BOX, sg.head0,
+                                (int32_t)(sg.q0 + i * g.tps), &q_full);
+          }
+        }
+        __syncwarp();
+        told = true;
+      };
+      if (ntile == 0) {
+        tell(true);
+        break;
+      }
+      for (int t = 0; t < ntile; ++t) {
         const int32_t pg = page, rw = row;
         lookup(t + 1, page, row);
         for (int kv = 0; kv < 2; ++kv, ++n) {
+          tell(2 * t + kv >= SLOTS);           // from there on a slot waits for this item's own tiles
           const uint32_t s = n % SLOTS;
           if (n >= SLOTS && ok && !mbar_wait_bounded(&kv_empty[s], (n / SLOTS - 1) & 1)) ok = false;
           __syncwarp();
@@ -163,11 +178,12 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
           }
         }
       }
-      at.unit += sg.ntile;
-      if (cut.tail)
-        at.it.s.b = -1;
-      else
-        paged_next(p, at);
+      tell(true);
+      if (me == 0 && lane == 0) {
+        if (!cut.head) paged_check_lens(p.pc, at.it.s);
+        if (cut.tail) paged_record(p, blockIdx.x, at, cut);
+      }
+      paged_advance(p, at, cut);
     }
    } else if (warp < 11) {
     // ------------------------------------------------ MMA of row tile i

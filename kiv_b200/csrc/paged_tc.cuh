@@ -96,6 +96,16 @@ __device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, i
 }
 }  // namespace tc
 
+// whether the phase of this parity is over, without waiting for it
+__device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+               : "=r"(ok)
+               : "r"(smem_u32(bar)), "r"(parity)
+               : "memory");
+  return ok != 0;
+}
+
 // one lane of the (converged) warp
 __device__ __forceinline__ bool elect_one() {
   uint32_t p;
@@ -135,16 +145,17 @@ __device__ __forceinline__ PtSeg pt_segment(const PagedPlan &p, const PagedSpot 
   cut = paged_segment(p, at);
   paged_range(p, at.it, at.rt, sg.lo, sg.hi);
   sg.hi = min(sg.hi, at.it.s.len);
-  sg.j00 = ((int64_t)sg.lo / PT_KEYS + cut.t0) * PT_KEYS;
+  sg.j00 = ((int64_t)(sg.lo / PT_KEYS) + cut.t0) * PT_KEYS;
   sg.ntile = cut.t1 - cut.t0;
   const int first = at.rt * p.tpt;
   sg.q0 = at.it.s.q0 + first;
   sg.tok = min(at.it.s.n - first, p.tpt);
   sg.nsub = sg.tok > tps ? 2 : 1;
   sg.base = p.q.causal ? at.it.base + first : at.it.s.len;
-  kvh = at.hp / p.hs;
-  sg.head0 = kvh * per + (at.hp % p.hs) * p.grp;
-  sg.heads = min(p.grp, per - (at.hp % p.hs) * p.grp);
+  const int part = p.hs == 1 ? 0 : at.hp % p.hs;
+  kvh = p.hs == 1 ? at.hp : at.hp / p.hs;
+  sg.head0 = kvh * per + part * p.grp;
+  sg.heads = min(p.grp, per - part * p.grp);
   sg.part = cut.head ? 2 * (int)blockIdx.x : cut.tail ? 2 * (int)blockIdx.x + 1 : -1;
   return sg;
 }

@@ -12,8 +12,9 @@
 // a time where they line up -- and walks the heads, RP_UN rows in flight.  A
 // lane holds two 16-byte vectors of a row, and for half-split pairs these are
 // the two sides of the same pairs: no exchange between lanes, and one cos and
-// sin per pair.  (One vector per lane, the other side by shuffles, took four
-// times the instructions and 53 us where this takes RP_TIME.)
+// sin per pair.  Measured: 2 x 4099 tokens of 28/4 x 128 (bf16, no norm, 139 MB)
+// 30 us, 4.6 TB/s; one vector per lane and the other side by shuffles took 2.2
+// times the instructions and 53 us, a block per token 82 us.
 #include <algorithm>
 
 #include "internal.h"
