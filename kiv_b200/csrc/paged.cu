@@ -72,21 +72,26 @@ static kiv_status check_paged_query(const kiv_paged *pc, const kiv_paged_query *
 constexpr int CC_KEYS = 64;
 constexpr int CC_THREADS = 256;
 
-template <int R>
-static size_t cc_smem(int D) {
-  return sizeof(float) * ((size_t)(R + 2 * CC_KEYS) * (D + 4) + (size_t)R * (CC_KEYS + 4));
+// fp32 rows up to 128: the next tile comes while this one is used
+template <typename T, int DM>
+__host__ __device__ constexpr int cc_buffers() { return sizeof(T) == 4 && DM <= 128 ? 2 : 1; }
+
+static size_t cc_smem(int rows, int D, int dtype) {
+  const int buffers = dtype == KIV_DTYPE_F32 && D <= 128 ? 2 : 1;
+  return sizeof(float) * ((size_t)(rows + buffers * 2 * CC_KEYS) * (D + 4) + (size_t)rows * (CC_KEYS + 4));
 }
 
 template <typename T, int R, int DM>
 __global__ void __launch_bounds__(CC_THREADS) paged_cc_kernel(const __grid_constant__ PagedPlan p) {
   constexpr int V = Elem<T>::V;
   constexpr int RPT = R / 16;          // rows per thread
+  constexpr int NBUF = cc_buffers<T, DM>();
   constexpr int DC = (DM + 63) / 64;   // 4-element slices of an output row per thread
   extern __shared__ float4 cc_dyn[];
-  __shared__ int64_t s_ko[CC_KEYS], s_vo[CC_KEYS];
+  __shared__ int64_t s_ko[3][CC_KEYS], s_vo[3][CC_KEYS];
   const int D = p.pc.head_dim, nv = D / V, ld = D + 4;
   float *sq = reinterpret_cast<float *>(cc_dyn);
-  float *sk = sq + R * ld, *sv = sk + CC_KEYS * ld, *sp = sv + CC_KEYS * ld;
+  float *const sk0 = sq + R * ld, *const sp = sk0 + NBUF * 2 * CC_KEYS * ld;   // [buffer][K, V][key]
   const int tr = threadIdx.x / 16, tc = threadIdx.x % 16;
   griddep_wait();
   PagedSpot at = paged_locate(p);              // every warp for itself
@@ -127,39 +132,77 @@ __global__ void __launch_bounds__(CC_THREADS) paged_cc_kernel(const __grid_const
 #pragma unroll
       for (int c = 0; c < DC; ++c) o[a][c] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    for (int t = g.t0; t < g.t1; ++t) {
-      const int64_t j0 = ((int64_t)lo / CC_KEYS + t) * CC_KEYS;
-      __syncthreads();                 // the previous step's readers are done
+    const int64_t j00 = ((int64_t)(lo / CC_KEYS) + g.t0) * CC_KEYS;
+    const int ntile = g.t1 - g.t0;
+    // where tile t's rows lie (-1: they read as zeros), a thread per key; three
+    // tiles' places are kept, so that the next one's are there when its copies go
+    auto places = [&](int t, int64_t &ko, int64_t &vo) {
+      const int64_t j = j00 + (int64_t)t * CC_KEYS + threadIdx.x;
+      ko = vo = -1;
+      if (t < ntile && threadIdx.x < CC_KEYS && j >= lo && j < hi) {
+        paged_key(p.pc, at.it.s.b, j, kvh, ko, vo);
+        if (ko < 0) paged_error(p.pc.errors, KIV_ERRBIT_BLOCK_TABLE);
+      }
+    };
+    auto keep = [&](int t, int64_t ko, int64_t vo) {
       if (threadIdx.x < CC_KEYS) {
-        const int64_t j = j0 + threadIdx.x;
-        int64_t ko = -1, vo = -1;
-        if (j >= lo && j < hi) {
-          paged_key(p.pc, at.it.s.b, j, kvh, ko, vo);
-          if (ko < 0) paged_error(p.pc.errors, KIV_ERRBIT_BLOCK_TABLE);
+        s_ko[t % 3][threadIdx.x] = ko;
+        s_vo[t % 3][threadIdx.x] = vo;
+      }
+    };
+    auto load = [&](int t) {                   // 16 threads per row
+      if (t < ntile) {
+        float *bk = sk0 + (t % NBUF) * 2 * CC_KEYS * ld, *bv = bk + CC_KEYS * ld;
+#pragma unroll
+        for (int y = 0; y < 2 * CC_KEYS / 16; ++y) {
+          const int r = (tr + 16 * y) % CC_KEYS;
+          const bool isv = tr + 16 * y >= CC_KEYS;
+          const int64_t off = isv ? s_vo[t % 3][r] : s_ko[t % 3][r];
+          const T *src = static_cast<const T *>(isv ? p.pc.v : p.pc.k) + (off < 0 ? 0 : off);
+          float *dst = (isv ? bv : bk) + r * ld;
+          for (int vi = tc; vi < nv; vi += 16) {
+            if constexpr (sizeof(T) == 4) {
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst + vi * V)), "l"(src + vi * V),
+                           "r"(off < 0 ? 0 : 16)
+                           : "memory");
+            } else {
+              float f[V];
+#pragma unroll
+              for (int e = 0; e < V; ++e) f[e] = 0.f;
+              if (off >= 0) Elem<T>::unpack(ld16(src + vi * V), f);
+#pragma unroll
+              for (int e = 0; e < V; e += 4) *reinterpret_cast<float4 *>(dst + vi * V + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+            }
+          }
         }
-        s_ko[threadIdx.x] = ko;
-        s_vo[threadIdx.x] = vo;
       }
-      __syncthreads();
-      for (int x = threadIdx.x; x < 2 * CC_KEYS * nv; x += CC_THREADS) {
-        const bool isv = x >= CC_KEYS * nv;
-        const int y = isv ? x - CC_KEYS * nv : x;
-        const int r = y / nv, vi = y - r * nv;
-        const int64_t off = isv ? s_vo[r] : s_ko[r];
-        float f[V];
-#pragma unroll
-        for (int e = 0; e < V; ++e) f[e] = 0.f;
-        if (off >= 0) Elem<T>::unpack(ld16(static_cast<const T *>(isv ? p.pc.v : p.pc.k) + off + vi * V), f);
-        float *d = (isv ? sv : sk) + r * ld + vi * V;
-#pragma unroll
-        for (int e = 0; e < V; ++e) d[e] = f[e];
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    __syncthreads();                           // the previous item's readers are done
+    int64_t nko, nvo;
+    for (int t = 0; t < 2; ++t) {
+      places(t, nko, nvo);
+      keep(t, nko, nvo);
+    }
+    __syncthreads();
+    load(0);
+    for (int t = 0; t < ntile; ++t) {
+      const int64_t j0 = j00 + (int64_t)t * CC_KEYS;
+      if (NBUF == 1 && t > 0) {
+        __syncthreads();                       // tile t - 1 is read
+        load(t);
       }
-      __syncthreads();
-      float s[RPT][4];
+      places(t + 2, nko, nvo);
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      __syncthreads();                         // tile t is there; with two buffers, tile t - 1 is read
+      if (NBUF == 2) load(t + 1);
+      const float *sk = sk0 + (t % NBUF) * 2 * CC_KEYS * ld, *sv = sk + CC_KEYS * ld;
+      float2 s2[RPT][4];                       // even and odd columns apart: two FMAs per instruction
 #pragma unroll
       for (int a = 0; a < RPT; ++a)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) s[a][c] = 0.f;
+        for (int c = 0; c < 4; ++c) s2[a][c] = make_float2(0.f, 0.f);
+#pragma unroll 4
       for (int d = 0; d < D; d += 4) {
         float4 kk[4];
 #pragma unroll
@@ -168,10 +211,17 @@ __global__ void __launch_bounds__(CC_THREADS) paged_cc_kernel(const __grid_const
         for (int a = 0; a < RPT; ++a) {
           const float4 qq = *reinterpret_cast<const float4 *>(sq + (tr * RPT + a) * ld + d);
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
-            s[a][c] = fmaf(qq.x, kk[c].x, fmaf(qq.y, kk[c].y, fmaf(qq.z, kk[c].z, fmaf(qq.w, kk[c].w, s[a][c]))));
+          for (int c = 0; c < 4; ++c) {
+            s2[a][c] = __ffma2_rn(make_float2(qq.x, qq.y), make_float2(kk[c].x, kk[c].y), s2[a][c]);
+            s2[a][c] = __ffma2_rn(make_float2(qq.z, qq.w), make_float2(kk[c].z, kk[c].w), s2[a][c]);
+          }
         }
       }
+      float s[RPT][4];
+#pragma unroll
+      for (int a = 0; a < RPT; ++a)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) s[a][c] = s2[a][c].x + s2[a][c].y;
 #pragma unroll
       for (int a = 0; a < RPT; ++a) {
         float mx = m[a];
@@ -208,7 +258,7 @@ __global__ void __launch_bounds__(CC_THREADS) paged_cc_kernel(const __grid_const
         }
       }
       __syncwarp();                    // a row's 16 threads are in one warp
-#pragma unroll 1
+#pragma unroll 2
       for (int j = 0; j < CC_KEYS; j += 4) {
         float4 pp[RPT];
 #pragma unroll
@@ -223,15 +273,16 @@ __global__ void __launch_bounds__(CC_THREADS) paged_cc_kernel(const __grid_const
 #pragma unroll
               for (int a = 0; a < RPT; ++a) {
                 const float e = jj == 0 ? pp[a].x : jj == 1 ? pp[a].y : jj == 2 ? pp[a].z : pp[a].w;
-                o[a][c].x = fmaf(e, vv.x, o[a][c].x);
-                o[a][c].y = fmaf(e, vv.y, o[a][c].y);
-                o[a][c].z = fmaf(e, vv.z, o[a][c].z);
-                o[a][c].w = fmaf(e, vv.w, o[a][c].w);
+                const float2 e2 = make_float2(e, e);
+                float2 lo2 = __ffma2_rn(e2, make_float2(vv.x, vv.y), make_float2(o[a][c].x, o[a][c].y));
+                float2 hi2 = __ffma2_rn(e2, make_float2(vv.z, vv.w), make_float2(o[a][c].z, o[a][c].w));
+                o[a][c] = make_float4(lo2.x, lo2.y, hi2.x, hi2.y);
               }
             }
           }
         }
       }
+      keep(t + 2, nko, nvo);                   // over tile t - 1's
     }
 #pragma unroll
     for (int a = 0; a < RPT; ++a) {
@@ -422,8 +473,7 @@ static PagedCall plan_call(const kiv_paged *pc, const kiv_paged_query *q) {
     c.kernel = PAGED_CC;
     const int rows = likely <= 16 ? 16 : 64;
     c.p = make_plan(pc, q, rows, CC_KEYS);
-    const size_t smem = rows == 16 ? cc_smem<16>(D) : cc_smem<64>(D);
-    c.blocks = sm_count() * (int)std::max<size_t>(1, std::min<size_t>(4, (220 * 1024) / (smem + 2048)));
+    c.blocks = sm_count() * (int)std::max<size_t>(1, std::min<size_t>(2, 233472 / (cc_smem(rows, D, pc->dtype) + 4608)));
   }
   c.cut_offset = (size_t)align_up((int64_t)2 * c.blocks * c.p.rows * partial_stride(D) * 4, 256);
   c.bytes = c.cut_offset + (size_t)align_up((int64_t)c.blocks * sizeof(PagedCut), 256);
@@ -432,7 +482,7 @@ static PagedCall plan_call(const kiv_paged *pc, const kiv_paged_query *q) {
 
 template <typename T, int R, int DM>
 static cudaError_t launch_cc(const PagedCall &c, cudaStream_t s) {
-  const size_t smem = cc_smem<R>(c.p.pc.head_dim);
+  const size_t smem = cc_smem(R, c.p.pc.head_dim, c.p.pc.dtype);
   cudaFuncSetAttribute(paged_cc_kernel<T, R, DM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   return launch_pdl(paged_cc_kernel<T, R, DM>, dim3((unsigned)c.blocks), dim3(CC_THREADS), smem, s, 1, c.p);
 }
