@@ -82,7 +82,7 @@ static size_t cc_smem(int rows, int D, int dtype) {
 }
 
 template <typename T, int R, int DM>
-__global__ void __launch_bounds__(CC_THREADS) paged_cc_kernel(const __grid_constant__ PagedPlan p) {
+__global__ void __launch_bounds__(CC_THREADS, DM <= 64 || (R == 16 && DM <= 128) ? 2 : 1) paged_cc_kernel(const __grid_constant__ PagedPlan p) {
   constexpr int V = Elem<T>::V;
   constexpr int RPT = R / 16;          // rows per thread
   constexpr int NBUF = cc_buffers<T, DM>();
@@ -473,7 +473,8 @@ static PagedCall plan_call(const kiv_paged *pc, const kiv_paged_query *q) {
     c.kernel = PAGED_CC;
     const int rows = likely <= 16 ? 16 : 64;
     c.p = make_plan(pc, q, rows, CC_KEYS);
-    c.blocks = sm_count() * (int)std::max<size_t>(1, std::min<size_t>(2, 233472 / (cc_smem(rows, D, pc->dtype) + 4608)));
+    const size_t most = D <= 64 || (rows == 16 && D <= 128) ? 2 : 1;       // as the kernel's launch bounds
+    c.blocks = sm_count() * (int)std::max<size_t>(1, std::min<size_t>(most, 233472 / (cc_smem(rows, D, pc->dtype) + 4608)));
   }
   c.cut_offset = (size_t)align_up((int64_t)2 * c.blocks * c.p.rows * partial_stride(D) * 4, 256);
   c.bytes = c.cut_offset + (size_t)align_up((int64_t)c.blocks * sizeof(PagedCut), 256);
