@@ -423,21 +423,33 @@ kiv_turn make_turn(const Tensor &rows, int64_t head_dim, const c10::optional<Ten
   return t;
 }
 
+// Rows as the kernels read them: last dim contiguous, 16-byte aligned -- the
+// tensor itself, or a copy.
+Tensor readable(const Tensor &x) {
+  const int64_t n = x.dim(), eb = x.element_size();
+  bool ok = n > 0 && x.numel() > 0 && x.stride(n - 1) == 1 && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
+  for (int64_t d = 0; ok && d + 1 < n; ++d) ok = x.size(d) == 1 || (x.stride(d) * eb) % 16 == 0;
+  return ok || x.numel() == 0 ? x : x.contiguous();
+}
+
 kiv_rows make_rows(const Tensor &x, const char *what) {
   TORCH_CHECK(x.dim() == 4 && x.stride(3) == 1, "kiv: ", what, " must be [B, H, Q, D] with a contiguous last dim");
   return kiv_rows{x.data_ptr(), step(x, 0), step(x, 1), step(x, 2), (int32_t)x.size(1), 0};
 }
 
-void qk_norm_rope(const Tensor &q, const c10::optional<Tensor> &k, const c10::optional<Tensor> &cos,
+void qk_norm_rope(const Tensor &q_in, const c10::optional<Tensor> &k_in, const c10::optional<Tensor> &cos,
                   const c10::optional<Tensor> &sin, const c10::optional<Tensor> &positions,
                   const c10::optional<Tensor> &pair_axes, bool interleaved, c10::optional<double> eps,
                   const c10::optional<Tensor> &q_weight, const c10::optional<Tensor> &k_weight, double weight_offset,
                   const Tensor &q_out, const c10::optional<Tensor> &k_out, const c10::optional<Tensor> &errors) {
-  c10::cuda::CUDAGuard g(q.device());
+  c10::cuda::CUDAGuard g(q_in.device());
+  const Tensor q = readable(q_in);
+  Tensor k;
+  if (const Tensor *t = given(k_in)) k = readable(*t);
   const kiv_rows qr = make_rows(q, "q"), qo = make_rows(q_out, "q_out");
   check_same(q, q_out, "q_out");
   TORCH_CHECK(q_out.sizes() == q.sizes() && q_out.scalar_type() == q.scalar_type(), "kiv: q_out must be like q");
-  const Tensor *kt = given(k), *kot = given(k_out);
+  const Tensor *kt = k.defined() ? &k : nullptr, *kot = given(k_out);
   TORCH_CHECK((kt != nullptr) == (kot != nullptr), "kiv: k and k_out come together");
   kiv_rows kr = {}, ko = {};
   if (kt) {
@@ -503,13 +515,14 @@ kiv_paged make_paged(const Tensor &rows, const Tensor &k_pages, const Tensor &v_
   return p;
 }
 
-void paged_append(const Tensor &k, const Tensor &v, const Tensor &k_pages, const Tensor &v_pages, const Tensor &table,
+void paged_append(const Tensor &k_in, const Tensor &v_in, const Tensor &k_pages, const Tensor &v_pages, const Tensor &table,
                   const Tensor &seq_lens, const Tensor &q_starts, const c10::optional<Tensor> &cos,
                   const c10::optional<Tensor> &sin, const c10::optional<Tensor> &positions,
                   const c10::optional<Tensor> &pair_axes, bool interleaved, c10::optional<double> eps,
                   const c10::optional<Tensor> &k_weight, double weight_offset, const c10::optional<Tensor> &errors) {
-  c10::cuda::CUDAGuard g(k.device());
-  check_same(k, v, "v");
+  c10::cuda::CUDAGuard g(k_in.device());
+  check_same(k_in, v_in, "v");
+  const Tensor k = readable(k_in), v = readable(v_in);
   const kiv_paged p = make_paged(k, k_pages, v_pages, table, seq_lens, q_starts, 0, errors);
   TORCH_CHECK(v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type() && v.stride(2) == 1 && k.size(1) == p.num_kv_heads,
               "kiv: new K/V rows must both be [tokens, Hkv, D]");
@@ -520,10 +533,11 @@ void paged_append(const Tensor &k, const Tensor &v, const Tensor &k_pages, const
         "paged_append");
 }
 
-void paged_attend(const Tensor &q, const Tensor &k_pages, const Tensor &v_pages, const Tensor &table, const Tensor &seq_lens,
+void paged_attend(const Tensor &q_in, const Tensor &k_pages, const Tensor &v_pages, const Tensor &table, const Tensor &seq_lens,
                   const Tensor &q_starts, double scaling, bool causal, int64_t window, double softcap, int64_t max_query_len,
                   const Tensor &out, const c10::optional<Tensor> &lse, const c10::optional<Tensor> &errors) {
-  c10::cuda::CUDAGuard g(q.device());
+  c10::cuda::CUDAGuard g(q_in.device());
+  const Tensor q = readable(q_in);
   const kiv_paged p = make_paged(q, k_pages, v_pages, table, seq_lens, q_starts, max_query_len, errors);
   check_same(q, out, "out");
   TORCH_CHECK(out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type() && out.stride(2) == 1, "kiv: out must be like q");

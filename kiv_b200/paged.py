@@ -35,16 +35,23 @@ from . import _native as nat
 from . import ops
 
 
-def _rows(x: torch.Tensor, what: str) -> torch.Tensor:
-    """Rows as the kernels read them: on a GPU, last dim contiguous, 16-byte aligned."""
-    if not x.is_cuda:
-        raise nat.KIVNativeError(f"{what} must be on a CUDA device (got {x.device}); the B200 kernels are the only "
+_ops: dict = {}
+
+
+def _run(name: str, rows: torch.Tensor, *args) -> None:
+    """One operator on the GPU of ``rows`` (the operator copies rows that are not 16-byte aligned)."""
+    if not rows.is_cuda:
+        raise nat.KIVNativeError(f"{name} needs tensors on a CUDA device (got {rows.device}); the B200 kernels are the only "
                                  "implementation")
-    nat.dtype_code(x.dtype)
-    mult = 16 // x.element_size()
-    if x.numel() and (x.stride(-1) != 1 or x.data_ptr() % 16 or any(s % mult for s, n in zip(x.stride()[:-1], x.shape) if n > 1)):
-        x = x.contiguous()
-    return x
+    op = _ops.get(name)
+    if op is None:
+        op = _ops[name] = getattr(ops.kiv(), name).default
+    try:
+        op(rows, *args)
+    except RuntimeError as e:
+        if "kiv" in str(e):
+            raise nat.KIVNativeError(str(e)) from e
+        raise
 
 
 def rotary_table(inv_freq: torch.Tensor, length: int, scaling: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
@@ -68,11 +75,11 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, cos: torch.Tensor | No
     already gathered per token.  A row whose position is outside the table comes out as NaN.
     Computed in float32 and rounded once.  ``out`` may be ``(q, k)`` themselves.
     """
-    q = _rows(q, "q")
-    if k is not None:
-        k = _rows(k, "k")
+    if out is None:                                  # outputs like the inputs, with a contiguous last dim
+        q = q if q.stride(-1) == 1 else q.contiguous()
+        k = k if k is None or k.stride(-1) == 1 else k.contiguous()
     q_out, k_out = out if out is not None else (torch.empty_like(q), None if k is None else torch.empty_like(k))
-    ops.call(ops.kiv().qk_norm_rope, q, k, cos, sin, positions, pair_axes, interleaved, eps, q_weight, k_weight,
+    _run("qk_norm_rope", q, k, cos, sin, positions, pair_axes, interleaved, eps, q_weight, k_weight,
              weight_offset, q_out, k_out, errors)
     return q_out, k_out
 
@@ -89,8 +96,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     in ``qk_norm_rope`` (``positions [tokens]`` or ``[A, tokens]``; without them by their place).  A token without a valid
     page, or with a position outside the table, is not written.
     """
-    k, v = _rows(k, "k"), _rows(v, "v")
-    ops.call(ops.kiv().paged_append, k, v, k_pages, v_pages, block_table, seq_lens, q_starts, cos, sin, positions,
+    _run("paged_append", k, v, k_pages, v_pages, block_table, seq_lens, q_starts, cos, sin, positions,
              pair_axes, interleaved, eps, k_weight, weight_offset, errors)
 
 
@@ -106,11 +112,11 @@ def paged_attend(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
     log-sum-exp of the scores ``[tokens, Hq]``; a row that sees no key gets 0 and -inf.  Keys without a valid page read
     as rows of zeros.  Rows of ``out`` and ``lse`` behind ``q_starts[-1]`` are left as they are.
     """
-    q = _rows(q, "q")
     if out is None:
+        q = q if q.stride(-1) == 1 else q.contiguous()
         out = torch.empty_like(q)
     lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
-    ops.call(ops.kiv().paged_attend, q, k_pages, v_pages, block_table, seq_lens, q_starts, scaling, causal, window, softcap,
+    _run("paged_attend", q, k_pages, v_pages, block_table, seq_lens, q_starts, scaling, causal, window, softcap,
              max_query_len, out, lse, errors)
     return (out, lse) if return_lse else out
 

@@ -439,3 +439,47 @@ def test_attend_windows_and_chunks_of_many_lengths_in_one_batch():
     for window, softcap in ((1500, 30.0), (200, 0.0), (0, 0.0)):
         check_attend(Case(new, lens, 16, 16, 96, 48, HF, seed=1), window=window, softcap=softcap)
         check_attend(Case(new[1:6], lens[1:6], 8, 1, 256, 24, BF, seed=2), window=window, softcap=softcap)
+
+
+def test_rows_of_any_strides():
+    """Misaligned and transposed rows are read through a copy; expanded ones as they are."""
+    base = torch.randn(2, 3, 5, 129, device=DEV, dtype=BF)
+    for q in (base[..., 1:], torch.randn(2, 3, 128, 5, device=DEV, dtype=BF).transpose(2, 3),
+              torch.randn(2, 1, 5, 128, device=DEV, dtype=BF).expand(2, 3, 5, 128)):
+        got, k = paged.qk_norm_rope(q, q, eps=1e-6)
+        want = ref_turn(q.double(), None, 1e-6, None, None, False)
+        for x in (got, k):
+            assert ((x.double() - want).abs() <= HALF[BF] * want.abs() + 1e-6 * want.abs().amax(-1, keepdim=True)).all()
+    c = Case([3, 40], [30, 90], 8, 2, 128, 16, BF)
+    want = paged.paged_attend(c.q, *c.args(), 0.1)
+    odd = torch.empty(43, 8, 129, device=DEV, dtype=BF)[..., 1:].copy_(c.q)
+    assert torch.equal(paged.paged_attend(odd, *c.args(), 0.1), want)
+    assert torch.equal(paged.paged_attend(c.q.transpose(1, 2).contiguous().transpose(1, 2), *c.args(), 0.1), want)
+    k1, v1 = (torch.randn(43, 2, 129, device=DEV, dtype=BF)[..., 1:] for _ in range(2))
+    paged.paged_append(k1, v1, *c.args())
+    assert torch.equal(c.kp[c.table[0, 29 // 16].long(), :, 29 % 16], k1[2])
+
+
+def test_refusals_of_tensors():
+    c = Case([3, 40], [30, 90], 8, 2, 128, 16, BF)
+    bad = [
+        lambda: paged.paged_attend(c.q, c.kp, c.vp, c.table.long(), c.d_lens, c.d_starts, 0.1),
+        lambda: paged.paged_attend(c.q, c.kp, c.vp, c.table, c.d_lens[:1], c.d_starts, 0.1),
+        lambda: paged.paged_attend(c.q, c.kp.float(), c.vp, c.table, c.d_lens, c.d_starts, 0.1),
+        lambda: paged.paged_attend(c.q, c.kp, c.vp, c.table.cpu(), c.d_lens, c.d_starts, 0.1),
+        lambda: paged.paged_attend(c.q[:, :7], *c.args(), 0.1),
+        lambda: paged.paged_attend(c.q, *c.args(), 0.1, window=-3),
+        lambda: paged.paged_attend(c.q, *c.args(), 0.1, window=3, causal=False),
+        lambda: paged.paged_attend(c.q, *c.args(), 0.1, out=c.q.float()),
+        lambda: paged.paged_attend(c.q[..., :64], *c.args(), 0.1),
+        lambda: paged.paged_append(c.k, c.v[:-1], *c.args()),
+        lambda: paged.paged_append(c.k, c.v, *c.args(), cos=torch.zeros(9, 64, device=DEV)),
+        lambda: paged.qk_norm_rope(c.q[None], None, torch.zeros(9, 65, device=DEV), torch.zeros(9, 65, device=DEV),
+                                   positions=torch.zeros(1, 8, device=DEV, dtype=torch.int64)),
+        lambda: paged.qk_norm_rope(c.q[None], None, torch.zeros(9, 64, device=DEV), torch.zeros(9, 64, device=DEV)),
+        lambda: paged.qk_norm_rope(c.q[None], None, q_weight=torch.zeros(128, device=DEV)),
+        lambda: paged.qk_norm_rope(c.q[None].double(), None, eps=1e-6),
+    ]
+    for f in bad:
+        with pytest.raises(nat.KIVNativeError):
+            f()
