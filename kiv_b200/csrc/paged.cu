@@ -341,9 +341,10 @@ __global__ void __launch_bounds__(CB_WARPS * 32) paged_combine_kernel(const __gr
   const int warp = (blockIdx.y * CB_WARPS + (threadIdx.x >> 5)), nwarps = gridDim.y * CB_WARPS;
   // parts: slot 2c + 1, then slot 2c' of the later blocks up to the last
   const int c0 = blockIdx.x, last = cut.last;
-  const int64_t stride = 2 * (int64_t)p.rows * partial_stride(D);
-  for (int x = warp; x < p.tpt * p.grp * slices; x += nwarps) {
-    const int r = x / slices, col = (x % slices) * 128 + 4 * lane;
+  const int64_t stride = 2 * 8 * (int64_t)partial_stride(D);       // two slots
+  const int tasks = min(p.tpt, cut.n - cut.rt * p.tpt) * p.grp * slices;   // rows that have tokens
+  for (int x = warp; x < tasks; x += nwarps) {
+    const int r = slices == 1 ? x : x / slices, slice = x - r * slices, col = slice * 128 + 4 * lane;
     int i, head;
     if (!paged_row(p, it, cut.hp, cut.rt, r, i, head)) continue;
     // lane k holds maximum and sum of part k of 32 at a time; the parts' values
@@ -400,7 +401,7 @@ __global__ void __launch_bounds__(CB_WARPS * 32) paged_combine_kernel(const __gr
       dst[2] = Elem<T>::from_f(acc.z * inv);
       dst[3] = Elem<T>::from_f(acc.w * inv);
     }
-    if (lane == 0 && x % slices == 0) paged_lse(p, it, i, head, mx, l);
+    if (lane == 0 && slice == 0) paged_lse(p, it, i, head, mx, l);
   }
 }
 
@@ -440,7 +441,7 @@ struct PagedCall {
   PagedPlan p;
   int blocks;
   size_t bytes;        // of its workspace
-  size_t cut_offset;
+  size_t part_offset;
 };
 
 // The kernel of a call and its tiling.  tcgen05 wherever TMA can bring the
@@ -476,8 +477,9 @@ static PagedCall plan_call(const kiv_paged *pc, const kiv_paged_query *q) {
     const size_t most = D <= 64 || (rows == 16 && D <= 128) ? 2 : 1;       // as the kernel's launch bounds
     c.blocks = sm_count() * (int)std::max<size_t>(1, std::min<size_t>(most, 233472 / (cc_smem(rows, D, pc->dtype) + 4608)));
   }
-  c.cut_offset = (size_t)align_up((int64_t)2 * c.blocks * c.p.rows * partial_stride(D) * 4, 256);
-  c.bytes = c.cut_offset + (size_t)align_up((int64_t)c.blocks * sizeof(PagedCut), 256);
+  c.p.slots = 2 * c.blocks;
+  c.part_offset = (size_t)align_up((int64_t)c.blocks * sizeof(PagedCut), 256);
+  c.bytes = c.part_offset + (size_t)align_up((int64_t)c.p.slots * c.p.rows * partial_stride(D) * 4, 256);
   return c;
 }
 
@@ -498,8 +500,8 @@ static cudaError_t launch_cc_r(const PagedCall &c, cudaStream_t s) {
 }
 
 static kiv_status run_call(PagedCall c, char *ws, cudaStream_t s) {
-  c.p.part = reinterpret_cast<float *>(ws);
-  c.p.cut = reinterpret_cast<PagedCut *>(ws + c.cut_offset);
+  c.p.cut = reinterpret_cast<PagedCut *>(ws);
+  c.p.part = reinterpret_cast<float *>(ws + c.part_offset);
   if (c.kernel == PAGED_MMA) return launch_paged_mma(c.p, c.blocks, s);
   if (c.kernel == PAGED_TC) return launch_paged_tc(c.p, c.blocks, s);
   cudaError_t e;

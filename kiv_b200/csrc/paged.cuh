@@ -84,8 +84,12 @@ struct PagedPlan {
   int kt;        // keys per key tile: a power of two
   int kt_log2;
   int rows;      // rows per part in the workspace: tpt * grp <= rows
-  float *part;   // [2 * G][rows][D + 2 (rounded to 4)]
-  struct PagedCut *cut;     // [G]
+  int slots;     // 2 G
+  // [rows / 8][slots][8][D + 2 (rounded to 4)]: the few rows of single tokens
+  // share a few memory pages over all slots, whose first touches cost most of a
+  // short call's join
+  float *part;
+  struct PagedCut *cut;     // [G], in front of them
 };
 
 // What block c says about the item it began and did not finish (b = -1: none)
@@ -225,9 +229,11 @@ __device__ __forceinline__ PagedSpot paged_locate(const PagedPlan &p) {
   const int per = (p.pc.batch + 31) / 32;
   const int b0 = lane * per, b1 = min(b0 + per, p.pc.batch);
   int64_t mine = 0;
+  PagedItems own;                                // with up to 32 sequences, the lane's only one
+  own.nrt = 0;
   for (int b = b0; b < b1; ++b) {
-    const PagedItems it = paged_items(p, b);
-    if (it.nrt > 0) mine += H * paged_line(p, it, it.nrt);
+    own = paged_items(p, b);
+    if (own.nrt > 0) mine += H * paged_line(p, own, own.nrt);
   }
   int64_t inc = mine;
 #pragma unroll
@@ -250,18 +256,21 @@ __device__ __forceinline__ PagedSpot paged_locate(const PagedPlan &p) {
   // the lane whose sequences hold the place, then the sequence among them
   int64_t at = r.unit - (inc - mine);
   const int owner = __ffs(__ballot_sync(KIV_FULL_MASK, at >= 0 && at < mine)) - 1;
-  int b = b0;
-  if (lane == owner) {
-    for (; b < b1; ++b) {
-      const PagedItems it = paged_items(p, b);
-      const int64_t n = it.nrt > 0 ? H * paged_line(p, it, it.nrt) : 0;
+  if (lane == owner && per > 1) {
+    for (int b = b0; b < b1; ++b) {
+      own = paged_items(p, b);
+      const int64_t n = own.nrt > 0 ? H * paged_line(p, own, own.nrt) : 0;
       if (at < n) break;
       at -= n;
     }
   }
-  b = __shfl_sync(KIV_FULL_MASK, b, owner);
   int64_t rem = __shfl_sync(KIV_FULL_MASK, at, owner);
-  r.it = paged_items(p, b);
+  r.it.s.b = __shfl_sync(KIV_FULL_MASK, own.s.b, owner);
+  r.it.s.q0 = __shfl_sync(KIV_FULL_MASK, own.s.q0, owner);
+  r.it.s.n = __shfl_sync(KIV_FULL_MASK, own.s.n, owner);
+  r.it.s.len = __shfl_sync(KIV_FULL_MASK, own.s.len, owner);
+  r.it.nrt = __shfl_sync(KIV_FULL_MASK, own.nrt, owner);
+  r.it.base = __shfl_sync(KIV_FULL_MASK, own.base, owner);
   const int64_t per_head = paged_line(p, r.it, r.it.nrt);
   r.hp = (int)paged_div(rem, per_head);
   rem -= (int64_t)r.hp * per_head;
@@ -342,7 +351,7 @@ __device__ __forceinline__ void paged_check_lens(const kiv_paged &pc, const Page
 }
 
 __device__ __forceinline__ float *paged_part(const PagedPlan &p, int64_t slot, int row) {
-  return p.part + (slot * p.rows + row) * partial_stride(p.pc.head_dim);
+  return p.part + (((int64_t)(row >> 3) * p.slots + slot) * 8 + (row & 7)) * partial_stride(p.pc.head_dim);
 }
 
 // Row r of an item's tile: token (in the sequence) and query head, or false
