@@ -501,6 +501,8 @@ typedef struct kiv_paged_query {
  * rows of zeros.  Rows of the pages past a sequence's length, and of pages no
  * row of a tile sees, never reach a result, whatever they hold.
  * Results do not depend on the order in which the GPU runs the blocks.
+ * fp32 rows are multiplied as sums of TF32 parts (22 bits of each product kept):
+ * an infinite element of a row that some query sees gives NaN.
  */
 KIV_API size_t kiv_paged_workspace_bytes(const kiv_paged *pc, const kiv_paged_query *q);
 KIV_API kiv_status kiv_paged_attend(const kiv_paged *pc, const kiv_paged_query *q, void *ws, size_t ws_bytes,

@@ -63,8 +63,7 @@ static kiv_status check_paged_query(const kiv_paged *pc, const kiv_paged_query *
 }
 
 // ---------------------------------------------------------------------------
-// CUDA-core kernel: fp32 rows (tensor cores would round them) and head
-// dimensions outside the tensor-core kernels' set.  R rows x 64 keys per
+// CUDA-core kernel: head dimensions outside the tensor-core kernels' set.  R rows x 64 keys per
 // step; 16 threads share a row, each with 4 keys of the scores and a sixteenth
 // of the output row.  Bound by the shared-memory reads that feed the FMAs
 // (a 4 x 4 register tile: 8 FMAs per 16 bytes read).
@@ -429,12 +428,12 @@ static PagedPlan make_plan(const kiv_paged *pc, const kiv_paged_query *q, int ro
   p.grp = (int)ceil_div(per, p.hs);
   p.tpt = p.tps = rows / p.grp;
   p.kt = kt;
-  p.kt_log2 = kt == 64 ? 6 : 7;
+  p.kt_log2 = kt == 32 ? 5 : kt == 64 ? 6 : 7;
   p.rows = rows;
   return p;
 }
 
-enum PagedKernel { PAGED_CC, PAGED_MMA, PAGED_TC };
+enum PagedKernel { PAGED_CC, PAGED_F32, PAGED_MMA, PAGED_TC };
 
 struct PagedCall {
   PagedKernel kernel;
@@ -448,8 +447,9 @@ struct PagedCall {
 // pages (paged_tc.cu): for single tokens too, 209 us against 249 (16 sequences of
 // 16 k keys, 32/8 x 128) and 62 against 84 (8/1 x 256) by the split kernel, which
 // keeps the pages of odd sizes and strides, the head dimensions 80 and 192 and
-// heads in groups above 128; CUDA cores for fp32 and what is left.  The lengths
-// are on the device, so the row tiles of the latter two go by what the host
+// heads in groups above 128; fp32 by split TF32 products (paged_f32.cu); CUDA
+// cores for what is left.  The lengths are on the device, so the row tiles of
+// all but the first go by what the host
 // knows: the rows of the longest sequence (max_query_len), or the mean.
 static PagedCall plan_call(const kiv_paged *pc, const kiv_paged_query *q) {
   PagedCall c;
@@ -470,6 +470,11 @@ static PagedCall plan_call(const kiv_paged *pc, const kiv_paged_query *q) {
     const int rows = likely <= 16 ? 16 : likely <= 32 ? 32 : 64;
     c.p = make_plan(pc, q, rows, 64);
     c.blocks = paged_mma_blocks(D, rows);
+  } else if (paged_f32_head(pc->dtype, D)) {
+    c.kernel = PAGED_F32;
+    const int rows = likely <= 16 ? 16 : likely <= 32 ? 32 : 64;
+    c.p = make_plan(pc, q, rows, 32);
+    c.blocks = paged_f32_blocks(D, rows);
   } else {
     c.kernel = PAGED_CC;
     const int rows = likely <= 16 ? 16 : 64;
@@ -503,6 +508,7 @@ static kiv_status run_call(PagedCall c, char *ws, cudaStream_t s) {
   c.p.cut = reinterpret_cast<PagedCut *>(ws);
   c.p.part = reinterpret_cast<float *>(ws + c.part_offset);
   if (c.kernel == PAGED_MMA) return launch_paged_mma(c.p, c.blocks, s);
+  if (c.kernel == PAGED_F32) return launch_paged_f32(c.p, c.blocks, s);
   if (c.kernel == PAGED_TC) return launch_paged_tc(c.p, c.blocks, s);
   cudaError_t e;
   if (c.p.pc.dtype == KIV_DTYPE_F32) e = launch_cc_r<float>(c, s);

@@ -123,7 +123,11 @@ __host__ __device__ inline int64_t floor_sum(int64_t count, uint32_t m, uint32_t
 }
 
 kiv_status launch_paged_combine(const PagedPlan &p, int blocks, cudaStream_t s);
-// few rows per key head, 16-bit rows (paged_mma.cu); plan rows 16, 32 or 64, kt 64
+// fp32 rows (paged_f32.cu); plan rows 16, 32 or 64, kt 32
+bool paged_f32_head(int dtype, int D);
+int paged_f32_blocks(int D, int rows);
+kiv_status launch_paged_f32(const PagedPlan &p, int blocks, cudaStream_t s);
+// 16-bit rows (paged_mma.cu); plan rows 16, 32 or 64, kt 64
 bool paged_mma_head(int dtype, int D);
 int paged_mma_blocks(int D, int rows);
 kiv_status launch_paged_mma(const PagedPlan &p, int blocks, cudaStream_t s);
