@@ -6,9 +6,14 @@
 // 2^-22 of each product, as small as the fp32 sums' own rounding.  Three
 // m16n8k8 MMAs stand against CUDA-core FMAs that needed 16 bytes of shared
 // memory for every 8 of them (paged.cu keeps that kernel for other head dimensions):
-// 181 us against 214 for 3 sequences of up to 130 tokens over 4096, 32/4 x 64,
-// and 132 against 225 for single tokens of 32 sequences of up to 8192.  An
+// 197 us against 214 for 3 sequences of up to 130 tokens over 4096, 32/4 x 64,
+// and 137 against 225 for single tokens of 32 sequences of up to 8192.  An
 // infinite element of a live row gives NaN (inf - inf in the split).
+//
+// The MMAs' own fp32 accumulation cuts instead of rounding: a sum carried through
+// thousands of them drifts towards zero (1e-4 after 20 k keys).  So they only sum
+// 16 columns of a score, or the keys of one tile, and what they give is added
+// to the score or the output by ordinary, rounding additions.
 //
 // The structure is that of paged_mma.cu: a ring of key tiles (32 keys), one
 // bulk copy per row, WM x WN = 4 warps over query rows and keys, the parts of a
@@ -199,6 +204,11 @@ __global__ void __launch_bounds__(MF_THREADS, F32Shape<D, 16 * WM>::BLOCKS) page
         uint32_t b[NK / 8][4];                 // of two steps of 8 columns
 #pragma unroll
         for (int n = 0; n < NK / 8; ++n) ldsm4f(b[n], kaddr + n * 8 * S::LD + k * 64);
+        float part[NK / 8][4];                 // of 16 columns: see above
+#pragma unroll
+        for (int n = 0; n < NK / 8; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) part[n][e] = 0.f;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           uint32_t a[4], ah[4], al[4];
@@ -206,8 +216,12 @@ __global__ void __launch_bounds__(MF_THREADS, F32Shape<D, 16 * WM>::BLOCKS) page
 #pragma unroll
           for (int e = 0; e < 4; ++e) split_tf32(a[e], ah[e], al[e]);
 #pragma unroll
-          for (int n = 0; n < NK / 8; ++n) mma_split(s[n], ah, al, b[n][2 * h], b[n][2 * h + 1]);
+          for (int n = 0; n < NK / 8; ++n) mma_split(part[n], ah, al, b[n][2 * h], b[n][2 * h + 1]);
         }
+#pragma unroll
+        for (int n = 0; n < NK / 8; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[n][e] += part[n][e];
       }
       const int64_t j0 = j00 + (int64_t)t * MF_KEYS;
       const bool open = j0 >= free_lo && j0 + MF_KEYS - 1 <= free_hi;
@@ -258,17 +272,23 @@ __global__ void __launch_bounds__(MF_THREADS, F32Shape<D, 16 * WM>::BLOCKS) page
           l[e >> 1] += s[n][e];
         }
       const float *vrow = reinterpret_cast<const float *>(mf_dyn + (n % STAGES) * S::STAGE + (MF_KEYS + wn * NK + 2 * tq) * S::LD) + g;
+      uint32_t ph[NK / 8][4], pl[NK / 8][4];   // k index t is key 2t, t + 4 is key 2t + 1
 #pragma unroll
       for (int c = 0; c < NK / 8; ++c) {
-        // k index t is key 2t, t + 4 is key 2t + 1
-        uint32_t ah[4], al[4];
-        split_tf32(__float_as_uint(s[c][0]), ah[0], al[0]);
-        split_tf32(__float_as_uint(s[c][2]), ah[1], al[1]);
-        split_tf32(__float_as_uint(s[c][1]), ah[2], al[2]);
-        split_tf32(__float_as_uint(s[c][3]), ah[3], al[3]);
+        split_tf32(__float_as_uint(s[c][0]), ph[c][0], pl[c][0]);
+        split_tf32(__float_as_uint(s[c][2]), ph[c][1], pl[c][1]);
+        split_tf32(__float_as_uint(s[c][1]), ph[c][2], pl[c][2]);
+        split_tf32(__float_as_uint(s[c][3]), ph[c][3], pl[c][3]);
+      }
 #pragma unroll
-        for (int d = 0; d < D / 8; ++d)
-          mma_split(o[d], ah, al, __float_as_uint(vrow[c * 8 * (S::LD / 4) + d * 8]), __float_as_uint(vrow[(c * 8 + 1) * (S::LD / 4) + d * 8]));
+      for (int d = 0; d < D / 8; ++d) {
+        float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < NK / 8; ++c)
+          mma_split(part, ph[c], pl[c], __float_as_uint(vrow[c * 8 * (S::LD / 4) + d * 8]),
+                    __float_as_uint(vrow[(c * 8 + 1) * (S::LD / 4) + d * 8]));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[d][e] += part[e];
       }
     }
     used += ntile;

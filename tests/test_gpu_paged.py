@@ -483,3 +483,15 @@ def test_refusals_of_tensors():
     for f in bad:
         with pytest.raises(nat.KIVNativeError):
             f()
+
+
+@pytest.mark.parametrize("D", [64, 256])
+def test_fp32_sums_over_many_keys_do_not_drift(D):
+    """Values around 1 over 20000 keys.  Sums that cut instead of rounding lose 2^-24 of themselves at each of thousands
+    of steps (1e-4).  Rounded ones walk: about 600 additions of at most 2^-24, four standard deviations 6e-6; with the
+    weights' own errors (scores of D products, exponential: below 3e-6, of both signs) 1e-5 covers them."""
+    c = Case([1, 3], [20000, 19000], 8, 1, D, 32, FP)
+    c.vp += 1
+    out = paged.paged_attend(c.q, *c.args(), D ** -0.5)
+    want, _ = ref_attend(c.q, c.kp, c.vp, c.table, c.lens, c.starts, D ** -0.5)
+    assert ((out.double() - want).abs() <= 1e-5 * want.abs().clamp(min=0.5)).all()
