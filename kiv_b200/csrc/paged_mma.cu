@@ -280,29 +280,38 @@ __global__ void __launch_bounds__(MM_THREADS, MmaShape<D, 16 * WM>::BLOCKS) page
           l[e >> 1] += s[n][e];
         }
       const uint32_t vaddr = vt + (wn * NK + (lane & 15)) * S::LD + (lane >> 4) * 16;
+      uint32_t a[NK / 16][4], ar[NK / 16][4];
 #pragma unroll
       for (int c = 0; c < NK / 16; ++c) {
-        uint32_t a[4], ar[4];
-        a[0] = pack2<BF>(s[2 * c][0], s[2 * c][1]);
-        a[1] = pack2<BF>(s[2 * c][2], s[2 * c][3]);
-        a[2] = pack2<BF>(s[2 * c + 1][0], s[2 * c + 1][1]);
-        a[3] = pack2<BF>(s[2 * c + 1][2], s[2 * c + 1][3]);
-        if (EXACT) {
-          ar[0] = pack2_rest<BF>(s[2 * c][0], s[2 * c][1], a[0]);
-          ar[1] = pack2_rest<BF>(s[2 * c][2], s[2 * c][3], a[1]);
-          ar[2] = pack2_rest<BF>(s[2 * c + 1][0], s[2 * c + 1][1], a[2]);
-          ar[3] = pack2_rest<BF>(s[2 * c + 1][2], s[2 * c + 1][3], a[3]);
-        }
 #pragma unroll
-        for (int d = 0; d < D / 16; ++d) {
+        for (int e = 0; e < 4; ++e) {
+          const float x = s[2 * c + (e >> 1)][2 * (e & 1)], y = s[2 * c + (e >> 1)][2 * (e & 1) + 1];
+          a[c][e] = pack2<BF>(x, y);
+          ar[c][e] = EXACT ? pack2_rest<BF>(x, y, a[c][e]) : 0u;
+        }
+      }
+      // The MMAs' accumulation cuts instead of rounding and would drift over
+      // many keys: they sum one tile, an ordinary addition the tiles.
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) {
+        float part[2][4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) part[0][e] = part[1][e] = 0.f;
+#pragma unroll
+        for (int c = 0; c < NK / 16; ++c) {
           uint32_t b[4];
           ldsm4t(b, vaddr + c * 16 * S::LD + d * 32);
-          mma16816<BF>(o[2 * d], a, b[0], b[1]);
-          mma16816<BF>(o[2 * d + 1], a, b[2], b[3]);
           if (EXACT) {
-            mma16816<BF>(o[2 * d], ar, b[0], b[1]);
-            mma16816<BF>(o[2 * d + 1], ar, b[2], b[3]);
+            mma16816<BF>(part[0], ar[c], b[0], b[1]);
+            mma16816<BF>(part[1], ar[c], b[2], b[3]);
           }
+          mma16816<BF>(part[0], a[c], b[0], b[1]);
+          mma16816<BF>(part[1], a[c], b[2], b[3]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          o[2 * d][e] += part[0][e];
+          o[2 * d + 1][e] += part[1][e];
         }
       }
     }

@@ -262,11 +262,12 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
         }
         if (more) wait(&kv_full[slot], phase);
         const uint64_t b = vd + vs * TILE16;
+        const bool fresh = (uint32_t)(t - first) / step % PT_FLUSH == 0;
         wait(&p_full[i], tiles & 1);
         tc::fence_after_sync();
         if (leader) {
 #pragma unroll
-          for (int k = 0; k < PT_HEAD / 16; ++k) tc::mma_f16_ta(to, ts + k * 8, b + k * S::BOXB, id_o, (t > first || k > 0) ? 1u : 0u);
+          for (int k = 0; k < PT_HEAD / 16; ++k) tc::mma_f16_ta(to, ts + k * 8, b + k * S::BOXB, id_o, (!fresh || k > 0) ? 1u : 0u);
         }
         wait(&p_tail[i], tiles & 1);
         tc::fence_after_sync();
@@ -318,6 +319,12 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
       const int64_t free_lo = max((int64_t)w.lo, p.q.window > 0 ? t0 + g.tps - p.q.window : (int64_t)0);
       const bool idle = (warp & 3) * 32 >= min(rows, (w.tok - sub * g.tps) * p.grp);   // a warp without rows keeps the beat
       float m = -INFINITY, l = 0.f;
+      // the row that the output moves to (PT_FLUSH), as of reference m_at; a
+      // whole item borrows the slot of a later cut one
+      const bool row = r < rows;
+      float *const acc = paged_part(p, w.part >= 0 ? w.part : 2 * (int)blockIdx.x + 1, twin ? grp * PT_ROWS + r : sub * rows + r);
+      bool moved = false;
+      float m_at = m;
       for (int t = first; t < w.ntile; t += step, ++tiles) {
         if (ok && !mbar_wait_bounded(&s_full[grp], tiles & 1)) ok = false;
         tc::fence_after_sync();
@@ -384,6 +391,11 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
             tc::st_32x16(to + x, o);
           }
         }
+        if (t > first && (uint32_t)(t - first) / step % PT_FLUSH == 0) {
+          pt_flush<D>(to, acc, !moved ? 0.f : m_at == m ? 1.f : ex2((m_at - m) * c), row);
+          moved = true;
+          m_at = m;
+        }
         const float2 c2 = make_float2(c, c);
         const float neg = m == -INFINITY ? 0.f : -m * c;
         const float2 n2 = make_float2(neg, neg);
@@ -420,11 +432,13 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
       // Twins: two groups hold the same rows, over the even and the odd key
       // tiles.  The second leaves maximum and sum in shared memory and its
       // output in TMEM, where the first one's threads reach the same lanes.
-      float f0 = 1.f, f1 = 0.f;
+      float f0 = 1.f, f1 = 0.f, fa = moved ? (m_at == m ? 1.f : ex2((m_at - m) * c)) : 0.f;
       if (twin) {
         if (grp == 1) {
           s_ml[0][r] = m;
           s_ml[1][r] = l;
+          // what has moved once moves whole, as of m
+          if (moved && !idle) pt_flush<D>(to, acc, m_at == m ? 1.f : ex2((m_at - m) * c), row);
           tc::fence_before_sync();
           asm volatile("bar.sync 1, 256;" ::: "memory");
           asm volatile("bar.sync 1, 256;" ::: "memory");     // read: the next item may overwrite it
@@ -439,11 +453,15 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
         m = top;
         l = l * f0 + l1 * f1;
       }
+      // of the other twin's row, and of what moved before
+      const bool moved1 = twin && w.ntile / 2 > PT_FLUSH;
+      const float *acc1 = paged_part(p, w.part >= 0 ? w.part : 2 * (int)blockIdx.x + 1, PT_ROWS + r);
       const float mnat = m * c * 0.693147181f;
       const bool whole = w.part < 0;
       const float inv = whole ? (l > 0.f ? 1.f / l : 0.f) : 1.f;
       f0 *= inv;
       f1 *= inv;
+      fa *= f0;
       const int head = w.head0 + gi;
       T *dst = static_cast<T *>(p.q.out) + (w.q0 + tok) * p.q.out_stride_t + head * p.q.out_stride_h;
       float *part = paged_part(p, w.part, sub * rows + r);
@@ -456,10 +474,18 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
           float *of = reinterpret_cast<float *>(o);
 #pragma unroll
           for (int y = 0; y < 32; ++y) of[y] = f0 == 0.f ? 0.f : of[y] * f0;   // nothing seen: what is there does not count
+          if (moved && have && fa != 0.f) {
+#pragma unroll
+            for (int y = 0; y < 32; ++y) of[y] = fmaf(acc[x + y], fa, of[y]);
+          }
           if (twin) {
             uint32_t o1[32];
             tc::ld_32x32(to + D + x, o1);
             tc::wait_ld32(o1);
+            if (moved1 && have) {
+#pragma unroll
+              for (int y = 0; y < 32; ++y) o1[y] = __float_as_uint(acc1[x + y]);
+            }
 #pragma unroll
             for (int y = 0; y < 32; ++y) of[y] = f1 == 0.f ? of[y] : fmaf(__uint_as_float(o1[y]), f1, of[y]);
           }

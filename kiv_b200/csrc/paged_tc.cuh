@@ -13,6 +13,11 @@ constexpr int PT_THREADS = 384;                // three warpgroups: two of softm
 // registers per thread: 168 at launch, (2 x 208 + 88) x 128 = 168 x 384 after the split
 constexpr int PT_REGS_SOFTMAX = 208, PT_REGS_OTHER = 88;
 constexpr int PT_HEAD = 96;                    // keys of a tile whose P V product begins before the rest of P is there
+// The tensor cores' accumulation cuts instead of rounding: a sum drifts towards
+// zero by 1e-7 of itself with every 16 keys (1.2e-3 after 200 k).  After this
+// many key tiles (1e-4) the output moves to a row of the workspace, added by
+// ordinary additions, and the products begin at zero again.
+constexpr int PT_FLUSH = 128;
 constexpr float PT_LAZY = 8.f;                 // growth (log2) that a row's reference may lag behind
 
 struct PagedTcGeom {
@@ -173,6 +178,32 @@ __device__ __forceinline__ void pt_lookup(const PagedPlan &p, const int32_t *tab
     if (page < 0 || page >= p.pc.num_pages) {
       paged_error(p.pc.errors, KIV_ERRBIT_BLOCK_TABLE);
       page = -1;
+    }
+  }
+}
+
+// Adds N columns of a row's output in TMEM to its row in the workspace: acc <-
+// acc f + o (f = 0: what is there does not count).  The whole warp; only lanes
+// with a row touch memory.
+template <int N>
+__device__ __forceinline__ void pt_flush(uint32_t to, float *acc, float f, bool row) {
+#pragma unroll 1
+  for (int x = 0; x < N; x += 16) {
+    uint32_t o[16];
+    tc::ld_32x16(to + x, o);
+    tc::wait_ld16(o);
+    if (row) {
+#pragma unroll
+      for (int y = 0; y < 16; y += 4) {
+        float4 *at = reinterpret_cast<float4 *>(acc + x + y);
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (f != 0.f) v = *at;
+        v.x = fmaf(v.x, f, __uint_as_float(o[y]));
+        v.y = fmaf(v.y, f, __uint_as_float(o[y + 1]));
+        v.z = fmaf(v.z, f, __uint_as_float(o[y + 2]));
+        v.w = fmaf(v.w, f, __uint_as_float(o[y + 3]));
+        *at = v;
+      }
     }
   }
 }

@@ -246,7 +246,7 @@ paged_tc256_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
 #pragma unroll
             for (int k = 0; k < 4; ++k)
               tc::mma_f16_ta(tmem + 2 * PT_KEYS, tmem + (tiles & 1) * PT_KEYS + (h * 4 + k) * 8, b + k * ((16 * 128) >> 4), id_o,
-                             (t > 0 || h > 0 || k > 0) ? 1u : 0u);
+                             (t % PT_FLUSH > 0 || h > 0 || k > 0) ? 1u : 0u);
             tc::commit(&kv_empty[r.slot(h)]);
           }
         }
@@ -288,6 +288,11 @@ paged_tc256_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
       const int64_t free_lo = max((int64_t)sg.lo, p.q.window > 0 ? (int64_t)sg.base + g.tps - p.q.window : (int64_t)0);
       const bool idle = (warp & 3) * 32 >= min(rows, sg.tok * p.grp);   // a warp without rows keeps the beat
       float m = -INFINITY, l = 0.f;
+      // the row that the output moves to, as in paged_tc.cu
+      const bool row = r < rows;
+      float *const acc = paged_part(p, sg.part >= 0 ? sg.part : 2 * (int)blockIdx.x + 1, r) + w * (P2_D / 2);
+      bool moved = false;
+      float m_at = m;
       vr.skip();                               // K(0)
       for (int t = 0; t < sg.ntile; ++t, ++tiles) {
         if (t + 1 < sg.ntile) vr.skip();       // K(t + 1); now at V(t)
@@ -364,6 +369,13 @@ paged_tc256_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
             tc::st_32x16(to + x, o);
           }
         }
+        if (t > 0 && t % PT_FLUSH == 0) {
+          wait(&pv_done[(tiles - 1) & 1], ((tiles - 1) >> 1) & 1);
+          tc::fence_after_sync();
+          pt_flush<P2_D / 2>(to, acc, !moved ? 0.f : m_at == m ? 1.f : ex2((m_at - m) * c), row);
+          moved = true;
+          m_at = m;
+        }
         const float2 c2 = make_float2(c, c);
         const float neg = m == -INFINITY ? 0.f : -m * c;
         const float2 n2 = make_float2(neg, neg);
@@ -396,6 +408,7 @@ paged_tc256_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
       const float mnat = m * c * 0.693147181f;
       const bool whole = sg.part < 0;
       const float inv = l > 0.f ? 1.f / l : 0.f;
+      const float fa = moved ? (m_at == m ? 1.f : ex2((m_at - m) * c)) : 0.f;
       const int head = sg.head0 + gi;
       T *dst = static_cast<T *>(p.q.out) + (sg.q0 + ti) * p.q.out_stride_t + head * p.q.out_stride_h + w * (P2_D / 2);
       float *part = paged_part(p, sg.part, r) + w * (P2_D / 2);
@@ -405,6 +418,10 @@ paged_tc256_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         tc::ld_32x32(to + x, o);
         tc::wait_ld32(o);
         if (!have) continue;
+        if (fa != 0.f) {
+#pragma unroll
+          for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(fmaf(acc[x + y], fa, __uint_as_float(o[y])));
+        }
         if (whole) {
 #pragma unroll
           for (int y = 0; y < 32; y += 8) {

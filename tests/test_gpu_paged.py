@@ -495,3 +495,30 @@ def test_fp32_sums_over_many_keys_do_not_drift(D):
     out = paged.paged_attend(c.q, *c.args(), D ** -0.5)
     want, _ = ref_attend(c.q, c.kp, c.vp, c.table, c.lens, c.starts, D ** -0.5)
     assert ((out.double() - want).abs() <= 1e-5 * want.abs().clamp(min=0.5)).all()
+
+
+@pytest.mark.parametrize("dtype,D,S,hq,hkv", [(HF, 128, 128, 8, 1), (HF, 64, 16, 8, 2), (HF, 256, 64, 8, 1), (BF, 96, 128, 4, 4), (HF, 128, 10, 8, 1)])
+def test_outputs_over_many_keys_do_not_drift(dtype, D, S, hq, hkv):
+    """Values around 1 over 60000 keys, so many items that blocks keep whole ones: prompts of two row tiles (the first
+    sequence) and of one.  The tensor cores cut their sums by about 2^-23 with every 16 keys (4e-4 here, most of an fp16
+    half step); moved on every 128 key tiles that is 1e-4.  The rounded weights add a walk, not a drift: of 60000
+    weights with errors of half a step of either sign, below 1e-4; the output's rounding is half a step.  In the mean of n outputs the drift stays, while n roundings, each
+    at most half a step h and even over it, leave a deviation of h / sqrt(3 n) (1.15e-4 for the 384 bf16 outputs of a
+    row here, 1e-5 for fp16): five of those are added."""
+    L = 60000
+    c = Case([700, 1, 5], [L, L - 3, L - 700], hq, hkv, D, S, dtype)
+    c.vp.mul_(0.25).add_(1)
+    out = paged.paged_attend(c.q, *c.args(), D ** -0.5, errors=c.errors)
+    rows = [0, 350, 699, 700, 701, 705]
+    at = [b for b, n in enumerate(c.new) for _ in range(n)]
+    for t in rows:
+        b = at[t]
+        n = c.lens[b] - c.starts[b + 1] + t + 1
+        j = torch.arange(n, device=DEV)
+        pg = c.table[b].long()[j // S]
+        k, v = (x[pg, :, j % S].double().repeat_interleave(hq // hkv, 1) for x in (c.kp, c.vp))
+        w = torch.softmax(torch.einsum("hd,lhd->hl", c.q[t].double(), k) * D ** -0.5, -1)
+        want = torch.einsum("hl,lhd->hd", w, v)
+        assert ((out[t].double() / want - 1).abs() <= HALF[dtype] + 2e-4).all(), t
+        assert (out[t].double() / want - 1).mean().abs() <= 1.5e-4 + 5 * HALF[dtype] / (3 * want.numel()) ** 0.5, t
+    assert int(c.errors) == 0
