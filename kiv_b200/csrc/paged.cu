@@ -63,10 +63,10 @@ static kiv_status check_paged_query(const kiv_paged *pc, const kiv_paged_query *
 }
 
 // ---------------------------------------------------------------------------
-// CUDA-core kernel: head dimensions outside the tensor-core kernels' set.  R rows x 64 keys per
-// step; 16 threads share a row, each with 4 keys of the scores and a sixteenth
-// of the output row.  Bound by the shared-memory reads that feed the FMAs
-// (a 4 x 4 register tile: 8 FMAs per 16 bytes read).
+// CUDA-core kernel: head dimensions outside the tensor-core kernels' set.
+// R rows x 64 keys per step; 16 threads share a row, each with 4 keys of the
+// scores and a sixteenth of the output row.  Bound by the shared-memory reads
+// that feed the FMAs (a 4 x 4 register tile: 8 FMAs per 16 bytes read).
 // ---------------------------------------------------------------------------
 constexpr int CC_KEYS = 64;
 constexpr int CC_THREADS = 256;
@@ -449,8 +449,8 @@ struct PagedCall {
 // keeps the pages of odd sizes and strides, the head dimensions 80 and 192 and
 // heads in groups above 128; fp32 by split TF32 products (paged_f32.cu); CUDA
 // cores for what is left.  The lengths are on the device, so the row tiles of
-// all but the first go by what the host
-// knows: the rows of the longest sequence (max_query_len), or the mean.
+// all but the first go by what the host knows: the rows of the longest sequence
+// (max_query_len), or the mean.
 static PagedCall plan_call(const kiv_paged *pc, const kiv_paged_query *q) {
   PagedCall c;
   const int D = pc->head_dim;

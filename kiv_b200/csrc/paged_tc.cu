@@ -25,7 +25,7 @@
 // products, so both are kept busy: per tile pair the tensor cores need 4 x 512
 // cycles (D = 128) and the 2 x 16384 exponentials 2048 cycles of the special
 // function units.  Measured: 4096 tokens over 36864 keys, 32/8 x 128: 2.2-2.4 ms,
-// 1.0-1.06 PFLOP/s at the power limit (1.3-1.4 GHz); with the softmax taken out
+// 0.92-1.06 PFLOP/s at the power limit (1.3-1.4 GHz); with the softmax taken out
 // the products alone take 1.6 ms.  One warp issuing both row tiles' products
 // took 3950 cycles per tile pair where this takes 3240.
 //
