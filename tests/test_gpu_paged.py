@@ -499,9 +499,8 @@ def test_fp32_sums_over_many_keys_do_not_drift(D):
 
 @pytest.mark.parametrize("dtype,D,S,hq,hkv", [(HF, 128, 128, 8, 1), (HF, 64, 16, 8, 2), (HF, 256, 64, 8, 1), (BF, 96, 128, 4, 4), (HF, 128, 10, 8, 1)])
 def test_outputs_over_many_keys_do_not_drift(dtype, D, S, hq, hkv):
-    """Values around 1 over 60000 keys, so many items that blocks keep whole ones: prompts of two row tiles (the first
-    sequence) and of one.  The tensor cores cut their sums by about 2^-23 with every 16 keys (4e-4 here, most of an fp16
-    half step); moved on every 128 key tiles that is 1e-4.  The rounded weights add a walk, not a drift: of 60000
+    """Values around 1 over 60000 keys, cut between the blocks.  The tensor cores cut their sums by about 2^-23 with
+    every 16 keys (4e-4 in one sum of all, most of an fp16 half step); over at most 128 key tiles that is 1e-4.  The rounded weights add a walk, not a drift: of 60000
     weights with errors of half a step of either sign, below 1e-4; the output's rounding is half a step.  In the mean of n outputs the drift stays, while n roundings, each
     at most half a step h and even over it, leave a deviation of h / sqrt(3 n) (1.15e-4 for the 384 bf16 outputs of a
     row here, 1e-5 for fp16): five of those are added."""
@@ -522,3 +521,35 @@ def test_outputs_over_many_keys_do_not_drift(dtype, D, S, hq, hkv):
         assert ((out[t].double() / want - 1).abs() <= HALF[dtype] + 2e-4).all(), t
         assert (out[t].double() / want - 1).mean().abs() <= 1.5e-4 + 5 * HALF[dtype] / (3 * want.numel()) ** 0.5, t
     assert int(c.errors) == 0
+
+
+@pytest.mark.parametrize("dtype,D,S,hq,hkv,new", [(HF, 128, 128, 8, 1, [5000, 1, 1000]), (HF, 256, 64, 8, 1, [2900, 100]), (BF, 96, 128, 1, 1, [40000]),
+                                                  (HF, 64, 16, 7, 1, [1, 5, 18] * 60), (HF, 128, 128, 4, 1, [1] * 200), (HF, 256, 64, 4, 2, [3] * 90)])
+def test_long_stretches_of_one_block_do_not_drift(dtype, D, S, hq, hkv, new):
+    """As above, with work for stretches of more than 128 key tiles in every block (256 where two groups of warps share
+    a sequence's tiles), whole items among them, and batches of few rows.  The sequences share their pages."""
+    L = 60000
+    g = torch.Generator(device=DEV).manual_seed(3)
+
+    def rows(*shape):
+        return torch.randn(shape, generator=g, device=DEV)
+
+    N = -(-L // S)
+    kp, vp, q = rows(N, hkv, S, D).to(dtype), (rows(N, hkv, S, D) / 4 + 1).to(dtype), rows(sum(new), hq, D).to(dtype)
+    lens = [L - 37 * (b % 5) for b in range(len(new))]
+    starts = [sum(new[:b]) for b in range(len(new) + 1)]
+    table = torch.arange(N, dtype=torch.int32, device=DEV).repeat(len(new), 1)
+    errors = torch.zeros(1, dtype=torch.int64, device=DEV)
+    ints = [torch.tensor(x, dtype=torch.int32, device=DEV) for x in (lens, starts)]
+    out, lse = paged.paged_attend(q, kp, vp, table, *ints, D ** -0.5, return_lse=True, errors=errors)
+    k, v = (x.transpose(1, 2).reshape(-1, hkv, D)[:L].double().repeat_interleave(hq // hkv, 1) for x in (kp, vp))
+    for b in sorted({0, 1, 2, len(new) // 2, len(new) - 1} & set(range(len(new)))):
+        for i in sorted({0, new[b] // 2, new[b] - 1}):
+            t, n = starts[b] + i, lens[b] - new[b] + i + 1
+            x = torch.einsum("hd,lhd->hl", q[t].double(), k[:n]) * D ** -0.5
+            want = torch.einsum("hl,lhd->hd", torch.softmax(x, -1), v[:n])
+            off = out[t].double() / want - 1
+            assert (off.abs() <= HALF[dtype] + 2e-4).all(), (t, off.abs().max())
+            assert off.mean().abs() <= 1.5e-4 + 5 * HALF[dtype] / (3 * want.numel()) ** 0.5, (t, off.mean())
+            assert (lse[t].double() - x.logsumexp(-1)).abs().max() <= 2e-5 * 12      # of values around 11.5
+    assert int(errors) == 0
