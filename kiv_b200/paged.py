@@ -24,7 +24,8 @@ could not follow -- they never read or write out of bounds.
 
 Every call runs on the current stream of its tensors' device, allocates its
 scratch from that stream's pool and raises ``KIVNativeError`` on refused
-arguments.  There is no CPU implementation.
+arguments.  There is no CPU implementation and no backward: inputs that require
+gradients are refused outside ``torch.no_grad()``.
 """
 
 from __future__ import annotations
@@ -54,6 +55,14 @@ def _run(name: str, rows: torch.Tensor, *args) -> None:
         raise
 
 
+def _refuse_gradients(name: str, *tensors: torch.Tensor | None) -> None:
+    """There is no backward: an input that needs one is refused, its gradient would be missing without a word."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise nat.KIVNativeError(f"{name} has no backward: call it under torch.no_grad() or on detached tensors")
+
+
 def rotary_table(inv_freq: torch.Tensor, length: int, scaling: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
     """cos and sin, float32 ``[length, len(inv_freq)]``, of positions 0 .. length - 1.  The angles are formed in 64
     bits: at position p one in 32 bits is off by up to p * 2^-24."""
@@ -75,6 +84,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, cos: torch.Tensor | No
     already gathered per token.  A row whose position is outside the table comes out as NaN.
     Computed in float32 and rounded once.  ``out`` may be ``(q, k)`` themselves.
     """
+    _refuse_gradients("qk_norm_rope", q, k, cos, sin, q_weight, k_weight)
     if out is None:                                  # outputs like the inputs, with a contiguous last dim
         q = q if q.stride(-1) == 1 else q.contiguous()
         k = k if k is None or k.stride(-1) == 1 else k.contiguous()
@@ -96,6 +106,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     in ``qk_norm_rope`` (``positions [tokens]`` or ``[A, tokens]``; without them by their place).  A token without a valid
     page, or with a position outside the table, is not written.
     """
+    _refuse_gradients("paged_append", k, v, k_pages, v_pages, cos, sin, k_weight)
     _run("paged_append", k, v, k_pages, v_pages, block_table, seq_lens, q_starts, cos, sin, positions,
              pair_axes, interleaved, eps, k_weight, weight_offset, errors)
 
@@ -112,6 +123,7 @@ def paged_attend(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
     log-sum-exp of the scores ``[tokens, Hq]``; a row that sees no key gets 0 and -inf.  Keys without a valid page read
     as rows of zeros.  Rows of ``out`` and ``lse`` behind ``q_starts[-1]`` are left as they are.
     """
+    _refuse_gradients("paged_attend", q, k_pages, v_pages)
     if out is None:
         q = q if q.stride(-1) == 1 else q.contiguous()
         out = torch.empty_like(q)

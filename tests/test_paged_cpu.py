@@ -229,3 +229,18 @@ def test_fused_rotation_stands_in_and_leaves_again():
         mw.uninstall()
     finally:
         module.apply_rotary_pos_emb = before
+
+
+def test_inputs_that_need_gradients_are_refused():
+    q, k = torch.zeros(1, 2, 1, 64), torch.zeros(1, 1, 1, 64)
+    w = torch.nn.Parameter(torch.ones(64))
+    rows, pages, ints = torch.zeros(1, 1, 64), torch.zeros(1, 1, 8, 64), torch.zeros(1, 1, dtype=torch.int32)
+    need = rows.clone().requires_grad_()
+    calls = [lambda: paged.qk_norm_rope(q.clone().requires_grad_(), k, eps=1e-6), lambda: paged.qk_norm_rope(q, k, eps=1e-6, k_weight=w),
+             lambda: paged.paged_append(rows, need, pages, pages, ints, ints[0], ints[0]),
+             lambda: paged.paged_attend(need, pages, pages, ints, ints[0], ints[0], 1.0)]
+    for call in calls:
+        with pytest.raises(nat.KIVNativeError, match="no backward"):
+            call()
+        with torch.no_grad(), pytest.raises(nat.KIVNativeError, match="CUDA device"):     # passes on to the next check
+            call()
