@@ -272,13 +272,18 @@ __global__ void __launch_bounds__(MM_THREADS, MmaShape<D, 16 * WM>::BLOCKS) page
         }
       }
       const float ms[2] = {m[0] == -INFINITY ? 0.f : m[0] * 1.44269504f, m[1] == -INFINITY ? 0.f : m[1] * 1.44269504f};
+      // a tile's weights first: one at a time, like ones would round the long sum
+      // the same way each time, and small ones not reach it at all
+      float sum[2] = {0.f, 0.f};
 #pragma unroll
       for (int n = 0; n < NK / 8; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           s[n][e] = ex2(fmaf(s[n][e], 1.44269504f, -ms[e >> 1]));
-          l[e >> 1] += s[n][e];
+          sum[e >> 1] += s[n][e];
         }
+      l[0] += sum[0];
+      l[1] += sum[1];
       const uint32_t vaddr = vt + (wn * NK + (lane & 15)) * S::LD + (lane >> 4) * 16;
       uint32_t a[NK / 16][4], ar[NK / 16][4];
 #pragma unroll
