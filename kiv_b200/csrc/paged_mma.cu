@@ -98,6 +98,9 @@ __global__ void __launch_bounds__(MM_THREADS, MmaShape<D, 16 * WM>::BLOCKS) page
   // second product (their rounding would be the largest error of the result);
   // with 64 rows the MMAs are no longer free and they are rounded once
   constexpr bool EXACT = WM == 1;
+  // fp16 weights are subnormal below 2^-14 and vanish below 2^-25 of the row's
+  // largest; 2^15 of them and of their sum keep those down to 2^-29 whole
+  constexpr float BIAS = BF ? 0.f : 15.f;
   constexpr bool QREG = D <= 128;              // query fragments stay in registers
   extern __shared__ __align__(128) uint8_t mm_dyn[];
   __shared__ uint64_t full[STAGES];
@@ -271,7 +274,10 @@ __global__ void __launch_bounds__(MM_THREADS, MmaShape<D, 16 * WM>::BLOCKS) page
           o[d][3] *= keep[1];
         }
       }
-      const float ms[2] = {m[0] == -INFINITY ? 0.f : m[0] * 1.44269504f, m[1] == -INFINITY ? 0.f : m[1] * 1.44269504f};
+      float shift[2];                          // fp16: rounded down, so that no weight passes 2^15
+#pragma unroll
+      for (int a = 0; a < 2; ++a)
+        shift[a] = m[a] == -INFINITY ? 0.f : BF ? -m[a] * 1.44269504f : __fmaf_rd(-m[a], 1.44269504f, BIAS);
       // a tile's weights first: one at a time, like ones would round the long sum
       // the same way each time, and small ones not reach it at all
       float sum[2] = {0.f, 0.f};
@@ -279,7 +285,7 @@ __global__ void __launch_bounds__(MM_THREADS, MmaShape<D, 16 * WM>::BLOCKS) page
       for (int n = 0; n < NK / 8; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          s[n][e] = ex2(fmaf(s[n][e], 1.44269504f, -ms[e >> 1]));
+          s[n][e] = ex2(fmaf(s[n][e], 1.44269504f, shift[e >> 1]));
           sum[e >> 1] += s[n][e];
         }
       l[0] += sum[0];
@@ -336,7 +342,7 @@ __global__ void __launch_bounds__(MM_THREADS, MmaShape<D, 16 * WM>::BLOCKS) page
 #pragma unroll
       for (int d = 0; d < D / 8; ++d) *reinterpret_cast<float2 *>(row + d * 8 + 2 * tq) = make_float2(o[d][2 * a], o[d][2 * a + 1]);
       if (tq == 0) {
-        row[D] = m[a];
+        row[D] = m[a] - BIAS * 0.693147181f;   // what the weights count in
         row[D + 1] = l[a];
       }
     }

@@ -31,9 +31,11 @@
 //
 // P (16-bit) overwrites S in TMEM and is the A operand from there; V is read
 // as an MN-major B operand straight from its row-major tile.  The output in
-// TMEM is rescaled only when a row's maximum has grown by more than 2^8 since
-// the reference it was scaled with (weights up to 256 are as exact as weights
-// up to 1: rounding is relative), which after the first tiles is almost never.
+// TMEM is rescaled only when a row's maximum has grown by more than 2^8 (fp16
+// 2^4) since the reference it was scaled with (weights up to 256 are as exact as
+// weights up to 1: rounding is relative), which after the first tiles is almost
+// never.  Rounding is relative as long as a weight is a normal number of its
+// type: fp16 weights carry a power of two for that (PT_BIAS).
 //
 // Key tiles that hold the end of a sequence (or keys before a window) may hold
 // anything in the dead rows, NaN too: scores there are replaced, not added to,
@@ -377,7 +379,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
         const float mn = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])));
         if (t == first) {
           m = mn;
-        } else if (__any_sync(KIV_FULL_MASK, (mn - m) * c > PT_LAZY)) {   // (-inf) - (-inf) is NaN: no growth
+        } else if (__any_sync(KIV_FULL_MASK, (mn - m) * c > PT_LAZY<BF>)) {   // (-inf) - (-inf) is NaN: no growth
           const float f = mn == -INFINITY ? 1.f : ex2((m - mn) * c);
           l *= f;
           m = mn;
@@ -397,7 +399,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
           m_at = m;
         }
         const float2 c2 = make_float2(c, c);
-        const float neg = m == -INFINITY ? 0.f : -m * c;
+        const float neg = pt_shift<BF>(m, c);
         const float2 n2 = make_float2(neg, neg);
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
@@ -456,7 +458,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
       // of the other twin's row, and of what moved before
       const bool moved1 = twin && w.ntile / 2 > PT_FLUSH;
       const float *acc1 = paged_part(p, w.part >= 0 ? w.part : 2 * (int)blockIdx.x + 1, PT_ROWS + r);
-      const float mnat = m * c * 0.693147181f;
+      const float mnat = pt_reference<BF>(m, c);
       const bool whole = w.part < 0;
       const float inv = whole ? (l > 0.f ? 1.f / l : 0.f) : 1.f;
       f0 *= inv;

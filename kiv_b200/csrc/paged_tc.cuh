@@ -18,7 +18,14 @@ constexpr int PT_HEAD = 96;                    // keys of a tile whose P V produ
 // many key tiles (1e-4) the output moves to a row of the workspace, added by
 // ordinary additions, and the products begin at zero again.
 constexpr int PT_FLUSH = 128;
-constexpr float PT_LAZY = 8.f;                 // growth (log2) that a row's reference may lag behind
+// Growth (log2) that a row's reference may lag behind, and the power of two by
+// which every weight, its sum and so the reference are scaled.  fp16 weights
+// would be subnormal below 2^-14 and vanish below 2^-25 of the reference while
+// the sum still counted them: one key 17 above a long tail lost the tail.  At
+// 2^11 they are whole down to 2^-25 and vanish below 2^-36 (128 k keys of those
+// hold 2e-6 of the row); the largest is 2^4 2^11, half of what fp16 holds.
+template <bool BF> constexpr float PT_LAZY = BF ? 8.f : 4.f;
+template <bool BF> constexpr float PT_BIAS = BF ? 0.f : 11.f;
 
 struct PagedTcGeom {
   int tps;       // tokens per row tile
@@ -127,6 +134,20 @@ __device__ __forceinline__ uint32_t pt_pack(float x, float y) {
     const __half2 h = __floats2half2_rn(x, y);
     return *reinterpret_cast<const uint32_t *>(&h);
   }
+}
+
+// What a row's score times c is added to in the exponent of its weight, m being
+// the reference.  Rounded down, so that no weight passes 2^(PT_LAZY + PT_BIAS)
+// however large the scores.
+template <bool BF>
+__device__ __forceinline__ float pt_shift(float m, float c) {
+  if (m == -INFINITY) return 0.f;
+  return BF ? -m * c : __fmaf_rd(-m, c, PT_BIAS<BF>);
+}
+// The natural logarithm of what the weights of reference m count in
+template <bool BF>
+__device__ __forceinline__ float pt_reference(float m, float c) {
+  return (BF ? m * c : m * c - PT_BIAS<BF>) * 0.693147181f;
 }
 
 // One segment of the block's stretch, as the TMA warp tells the others.

@@ -353,7 +353,7 @@ paged_tc256_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         mn = fmaxf(mn, s_max[tiles & 1][w ^ 1][r]);
         if (t == 0) {
           m = mn;
-        } else if (__any_sync(KIV_FULL_MASK, (mn - m) * c > PT_LAZY)) {   // the same in both groups
+        } else if (__any_sync(KIV_FULL_MASK, (mn - m) * c > PT_LAZY<BF>)) {   // the same in both groups
           const float f = mn == -INFINITY ? 1.f : ex2((m - mn) * c);
           l *= f;
           m = mn;
@@ -377,7 +377,7 @@ paged_tc256_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
           m_at = m;
         }
         const float2 c2 = make_float2(c, c);
-        const float neg = m == -INFINITY ? 0.f : -m * c;
+        const float neg = pt_shift<BF>(m, c);
         const float2 n2 = make_float2(neg, neg);
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         uint32_t pk[COLS / 2];
@@ -405,7 +405,7 @@ paged_tc256_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
       l += sum_at[w ^ 1][r];                   // a + b in both groups: the same
       wait(&pv_done[(tiles - 1) & 1], ((tiles - 1) >> 1) & 1);
       tc::fence_after_sync();
-      const float mnat = m * c * 0.693147181f;
+      const float mnat = pt_reference<BF>(m, c);
       const bool whole = sg.part < 0;
       const float inv = l > 0.f ? 1.f / l : 0.f;
       const float fa = moved ? (m_at == m ? 1.f : ex2((m_at - m) * c)) : 0.f;

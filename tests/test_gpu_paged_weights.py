@@ -60,3 +60,40 @@ def test_small_weights_reach_the_sum_of_a_large_one(dtype, D, S, tile, heads):
     want = 17.5 + math.log1p((L - 1) * math.exp(-17.5))
     assert (lse.double() - want).abs().max() <= off + 2e-6 * 17.5
     assert (out[..., 0].double() * math.exp(want - 17.5) - 1).abs().max() <= off + 2e-5 + HALF[dtype]
+
+
+@pytest.mark.parametrize("D,S,hq,new", [
+    (128, 128, 8, [1] * 200), (64, 16, 7, [18, 1, 5] * 60), (96, 48, 1, [40000]), (128, 16, 8, [5000, 1, 900]),   # tcgen05
+    (256, 64, 8, [3] * 90), (256, 128, 8, [2900, 100]),
+    (80, 16, 8, [1] * 500), (80, 16, 8, [3] * 300), (128, 10, 8, [40] * 300)])                                    # warp-level MMAs
+def test_fp16_weights_far_below_the_largest_count(D, S, hq, new):
+    """One key with value 0 scores 17.5 above a tail of 60000 whose values are around 1: the result is the tail's share,
+    1.5e-3.  Each weight is rounded to fp16, at most half a step h = 2^-11 of itself while it is a normal number (2 h for
+    the few that are not), the output to h of itself, the tensor cores' cutting sums over at most 128 key tiles 1e-4 (as in the drift
+    tests), and the sum of the weights, near 1, is off by at most half a step at each of up to 940 key tiles, 6e-5; scores
+    near 17.5 in fp32 and the exponential, 1e-5."""
+    L = 60000
+    g = torch.Generator(device=DEV).manual_seed(7)
+    kp, vp, table = shared_pages(L, S, 1, D, HF, len(new))
+    k, v = (x.view(-1, S, D)[:, :, :].reshape(-1, D) for x in (kp, vp))
+    k[:, 1] = (torch.randn(k.shape[0], generator=g, device=DEV) * 0.5).to(HF)
+    v.copy_((torch.randn(v.shape, generator=g, device=DEV) / 4 + 1).to(HF))
+    k[0], v[0] = 0, 0
+    k[0, 0] = 17.5
+    q = torch.zeros(sum(new), hq, D, dtype=HF, device=DEV)
+    q[..., 0] = 1
+    q[..., 1] = torch.rand(q.shape[:2], generator=g, device=DEV).to(HF)
+    lens = [L - 37 * (b % 5) for b in range(len(new))]
+    starts = [sum(new[:b]) for b in range(len(new) + 1)]
+    errors = torch.zeros(1, dtype=torch.int64, device=DEV)
+    out, lse = paged.paged_attend(q, kp, vp, table, *ints(lens, starts), 1.0, max_query_len=max(new), return_lse=True, errors=errors)
+    h = HALF[HF]
+    for b in sorted({0, 1, len(new) // 2, len(new) - 1} & set(range(len(new)))):
+        for i in sorted({0, new[b] // 2, new[b] - 1}):
+            t, n = starts[b] + i, lens[b] - new[b] + i + 1
+            x = q[t].double() @ k[:n].double().T
+            want = torch.softmax(x, -1) @ v[:n].double()
+            assert want.abs().max() < 5e-3
+            assert ((out[t].double() / want - 1).abs() <= 3 * h + 2e-4).all(), (t, (out[t].double() / want - 1).abs().max())
+            assert (lse[t].double() - x.logsumexp(-1)).abs().max() <= 2e-5 * 17.5
+    assert int(errors) == 0
