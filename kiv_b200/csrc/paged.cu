@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(CC_THREADS, DM <= 64 || (R == 16 && DM <= 128)
       int i, head;
       paged_row(p, at.it, at.hp, at.rt, r, i, head);
       if (!g.head && !g.tail) {
-        const float inv = l[a] > 0.f ? 1.f / l[a] : 0.f;
+        const float inv = paged_inv(l[a]);
         T *dst = paged_out<T>(p, at.it, i, head);
 #pragma unroll
         for (int c = 0; c < DC; ++c) {
@@ -392,7 +392,7 @@ __global__ void __launch_bounds__(CB_WARPS * 32) paged_combine_kernel(const __gr
         }
       }
     }
-    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const float inv = paged_inv(l);
     if (col < D) {
       T *dst = paged_out<T>(p, it, i, head) + col;
       dst[0] = Elem<T>::from_f(acc.x * inv);

@@ -413,8 +413,13 @@ template <typename T>
 __device__ __forceinline__ T *paged_out(const PagedPlan &p, const PagedItems &it, int i, int head) {
   return static_cast<T *>(p.q.out) + (it.s.q0 + i) * p.q.out_stride_t + head * p.q.out_stride_h;
 }
+// A row's factor and log-sum-exp from its maximum and sum.  A row that has seen
+// no key has the sum 0; a sum that is NaN (a NaN in the query or in a key that it
+// sees) stays one.
+__device__ __forceinline__ float paged_inv(float l) { return l == 0.f ? 0.f : 1.f / l; }
+__device__ __forceinline__ float paged_log(float m, float l) { return l == 0.f ? -INFINITY : m + logf(l); }
 __device__ __forceinline__ void paged_lse(const PagedPlan &p, const PagedItems &it, int i, int head, float m, float l) {
-  if (p.q.lse) p.q.lse[(it.s.q0 + i) * p.q.num_query_heads + head] = l > 0.f ? m + logf(l) : -INFINITY;
+  if (p.q.lse) p.q.lse[(it.s.q0 + i) * p.q.num_query_heads + head] = paged_log(m, l);
 }
 
 // Element offsets of key j's rows in k and v, or -1 where it has no page

@@ -338,7 +338,7 @@ __global__ void __launch_bounds__(MF_THREADS, F32Shape<D, 16 * WM>::BLOCKS) page
         for (int e = 0; e < 8; ++e) acc[e] = fmaf(row[c + e], f, acc[e]);
       }
       if (!sg.head && !sg.tail) {
-        const float inv = ll > 0.f ? 1.f / ll : 0.f;
+        const float inv = paged_inv(ll);
 #pragma unroll
         for (int e = 0; e < 8; ++e) acc[e] *= inv;
         T *dst = paged_out<T>(p, at.it, i, head) + c;

@@ -460,7 +460,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
       const float *acc1 = paged_part(p, w.part >= 0 ? w.part : 2 * (int)blockIdx.x + 1, PT_ROWS + r);
       const float mnat = pt_reference<BF>(m, c);
       const bool whole = w.part < 0;
-      const float inv = whole ? (l > 0.f ? 1.f / l : 0.f) : 1.f;
+      const float inv = whole ? paged_inv(l) : 1.f;
       f0 *= inv;
       f1 *= inv;
       fa *= f0;
@@ -502,7 +502,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
         }
         if (have) {
           if (whole) {
-            if (p.q.lse) p.q.lse[(w.q0 + tok) * p.q.num_query_heads + head] = l > 0.f ? mnat + logf(l) : -INFINITY;
+            if (p.q.lse) p.q.lse[(w.q0 + tok) * p.q.num_query_heads + head] = paged_log(mnat, l);
           } else {
             part[D] = mnat;
             part[D + 1] = l;

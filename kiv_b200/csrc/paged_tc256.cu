@@ -407,7 +407,7 @@ paged_tc256_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
       tc::fence_after_sync();
       const float mnat = pt_reference<BF>(m, c);
       const bool whole = sg.part < 0;
-      const float inv = l > 0.f ? 1.f / l : 0.f;
+      const float inv = paged_inv(l);
       const float fa = moved ? (m_at == m ? 1.f : ex2((m_at - m) * c)) : 0.f;
       const int head = sg.head0 + gi;
       T *dst = static_cast<T *>(p.q.out) + (sg.q0 + ti) * p.q.out_stride_t + head * p.q.out_stride_h + w * (P2_D / 2);
@@ -439,7 +439,7 @@ paged_tc256_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
       }
       if (have && w == 0) {
         if (whole) {
-          if (p.q.lse) p.q.lse[(sg.q0 + ti) * p.q.num_query_heads + head] = l > 0.f ? mnat + logf(l) : -INFINITY;
+          if (p.q.lse) p.q.lse[(sg.q0 + ti) * p.q.num_query_heads + head] = paged_log(mnat, l);
         } else {
           part[P2_D] = mnat;
           part[P2_D + 1] = l;

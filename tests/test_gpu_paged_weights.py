@@ -97,3 +97,23 @@ def test_fp16_weights_far_below_the_largest_count(D, S, hq, new):
             assert ((out[t].double() / want - 1).abs() <= 3 * h + 2e-4).all(), (t, (out[t].double() / want - 1).abs().max())
             assert (lse[t].double() - x.logsumexp(-1)).abs().max() <= 2e-5 * 17.5
     assert int(errors) == 0
+
+
+@pytest.mark.parametrize("dtype,D,S", [(BF, 128, 16), (HF, 64, 16), (BF, 256, 32), (BF, 80, 16), (HF, 128, 10), (FP, 64, 16), (FP, 40, 8)])
+@pytest.mark.parametrize("n,L", [(1, 300), (3, 70), (90, 200), (1, 30000), (200, 20000)])
+def test_nan_in_a_live_row_reaches_the_results_it_belongs_to(dtype, D, S, n, L):
+    """A NaN query gives a NaN row, a NaN key a NaN for every row that sees it; nothing else changes."""
+    c = Case([n, n], [L, L], 4, 2, D, S, dtype, seed=n)
+    t = n // 2
+    clean, clse = paged.paged_attend(c.q, *c.args(), D ** -0.5, return_lse=True)
+    c.q[t, 1, 3] = math.nan                                     # sequence 0, one token, one head
+    j = L - n + t                                               # sequence 1: the key of its new token t, key head 1
+    pg = int(c.table[1, j // S])
+    c.kp[pg, 1, j % S, 5] = math.nan
+    out, lse = paged.paged_attend(c.q, *c.args(), D ** -0.5, return_lse=True, errors=c.errors)
+    bad = torch.zeros(2 * n, 4, dtype=torch.bool, device=DEV)
+    bad[t, 1] = True
+    bad[n + t:, 2:] = True
+    assert torch.isnan(out[bad]).all() and torch.isnan(lse[bad]).all()
+    assert torch.equal(out[~bad], clean[~bad]) and torch.equal(lse[~bad], clse[~bad])
+    assert int(c.errors) == 0
