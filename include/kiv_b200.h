@@ -417,7 +417,8 @@ KIV_API kiv_status kiv_attend_exchange_merge(const kiv_store *st, const kiv_quer
  */
 typedef struct kiv_paged {
   int32_t batch, num_kv_heads, head_dim, page_size, dtype;
-  int32_t max_query_len;    /* largest n_b if the host knows it, else 0: picks kernels, never results */
+  int32_t max_query_len;    /* largest n_b if the host knows it, else 0: picks tilings (the order
+                               of fp32 sums), never which keys count or how exactly */
   int64_t num_pages;
   void *k, *v;
   int64_t k_stride_p, k_stride_h, k_stride_t;   /* elements */

@@ -94,10 +94,12 @@ __global__ void __launch_bounds__(MM_THREADS, MmaShape<D, 16 * WM>::BLOCKS) page
   constexpr int NK = MM_KEYS / WN;             // keys per warp and tile
   constexpr int CH = D / 8;                    // 16-byte chunks per row
   constexpr int STAGES = S::STAGES;
-  // decode is bound by memory, so the probabilities keep 16 more bits in a
-  // second product (their rounding would be the largest error of the result);
-  // with 64 rows the MMAs are no longer free and they are rounded once
-  constexpr bool EXACT = WM == 1;
+  // The probabilities keep their type's bits twice, in a second product: their
+  // rounding would be the largest error of the result.  With 16 rows (bound by
+  // memory) it is free; with 64 rows it takes 4 to 19 % (2048 tokens over 16384,
+  // 32/8 x 80: 2.91 ms from 2.79; x 192: 7.7 from 6.8).  All row counts do it, as
+  // a call's tiling goes by what the host knows of the lengths, and that must not
+  // decide how exact a row is.
   // fp16 weights are subnormal below 2^-14 and vanish below 2^-25 of the row's
   // largest; 2^15 of them and of their sum keep those down to 2^-29 whole
   constexpr float BIAS = BF ? 0.f : 15.f;
@@ -298,7 +300,7 @@ __global__ void __launch_bounds__(MM_THREADS, MmaShape<D, 16 * WM>::BLOCKS) page
         for (int e = 0; e < 4; ++e) {
           const float x = s[2 * c + (e >> 1)][2 * (e & 1)], y = s[2 * c + (e >> 1)][2 * (e & 1) + 1];
           a[c][e] = pack2<BF>(x, y);
-          ar[c][e] = EXACT ? pack2_rest<BF>(x, y, a[c][e]) : 0u;
+          ar[c][e] = pack2_rest<BF>(x, y, a[c][e]);
         }
       }
       // The MMAs' accumulation cuts instead of rounding and would drift over
@@ -312,10 +314,8 @@ __global__ void __launch_bounds__(MM_THREADS, MmaShape<D, 16 * WM>::BLOCKS) page
         for (int c = 0; c < NK / 16; ++c) {
           uint32_t b[4];
           ldsm4t(b, vaddr + c * 16 * S::LD + d * 32);
-          if (EXACT) {
-            mma16816<BF>(part[0], ar[c], b[0], b[1]);
-            mma16816<BF>(part[1], ar[c], b[2], b[3]);
-          }
+          mma16816<BF>(part[0], ar[c], b[0], b[1]);
+          mma16816<BF>(part[1], ar[c], b[2], b[3]);
           mma16816<BF>(part[0], a[c], b[0], b[1]);
           mma16816<BF>(part[1], a[c], b[2], b[3]);
         }

@@ -119,9 +119,10 @@ def paged_attend(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
 
     ``causal``: new token i of the n of sequence b sees keys ``j <= seq_lens[b] - n + i``, with ``window`` only the last
     ``window`` of them; otherwise all.  ``softcap``: scores ``c * tanh(s / c)``.  ``max_query_len``: the largest n, where
-    the host knows it (chooses kernels, never changes which keys count).  With ``return_lse`` also the float32
-    log-sum-exp of the scores ``[tokens, Hq]``; a row that sees no key gets 0 and -inf.  Keys without a valid page read
-    as rows of zeros.  Rows of ``out`` and ``lse`` behind ``q_starts[-1]`` are left as they are.
+    the host knows it (chooses tilings, and so the order of fp32 sums, never which keys count or how exactly).  With
+    ``return_lse`` also the float32 log-sum-exp of the scores ``[tokens, Hq]``; a row that sees no key gets 0 and -inf.
+    Keys without a valid page read as rows of zeros.  Rows of ``out`` and ``lse`` behind ``q_starts[-1]`` are left as they
+    are.
     """
     _refuse_gradients("paged_attend", q, k_pages, v_pages)
     if out is None:

@@ -117,3 +117,19 @@ def test_nan_in_a_live_row_reaches_the_results_it_belongs_to(dtype, D, S, n, L):
     assert torch.isnan(out[bad]).all() and torch.isnan(lse[bad]).all()
     assert torch.equal(out[~bad], clean[~bad]) and torch.equal(lse[~bad], clse[~bad])
     assert int(c.errors) == 0
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("D,S", [(80, 16), (192, 16), (128, 10), (64, 7), (256, 12)])
+def test_the_hint_of_the_longest_query_changes_no_precision(dtype, D, S):
+    """The warp-level kernels go by max_query_len (16, 32 or 64 rows) or the mean.  Whatever it says, few keys or many:
+    the weights keep twice the rows' bits, so an output is off by its own rounding, half a step, and 2e-5 of the largest
+    value for fp32 sums (a weight rounded once would be off by up to half a step of the largest value)."""
+    for new, lens in (([1, 2, 1], [3, 2, 5]), ([5, 1, 40], [9, 300, 77])):
+        c = Case(new, lens, 8, 2, D, S, dtype, seed=D)
+        want, _ = ref_attend(c.q, c.kp, c.vp, c.table, c.lens, c.starts, D ** -0.5)
+        for hint in (0, 1, 5, 12, 40, 4000):
+            got = paged.paged_attend(c.q, *c.args(), D ** -0.5, max_query_len=hint, errors=c.errors).double()
+            err = (got - want).abs() - HALF[dtype] * want.abs() - 2e-5 * c.v_live
+            assert (err <= 0).all(), (hint, err.max())
+        assert int(c.errors) == 0
