@@ -429,7 +429,7 @@ Tensor readable(const Tensor &x) {
   const int64_t n = x.dim(), eb = x.element_size();
   bool ok = n > 0 && x.numel() > 0 && x.stride(n - 1) == 1 && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
   for (int64_t d = 0; ok && d + 1 < n; ++d) ok = x.size(d) == 1 || (x.stride(d) * eb) % 16 == 0;
-  return ok || x.numel() == 0 ? x : x.contiguous();
+  return ok || x.numel() == 0 ? x : x.clone(at::MemoryFormat::Contiguous);   // a contiguous one may be misaligned too
 }
 
 kiv_rows make_rows(const Tensor &x, const char *what) {

@@ -1,0 +1,55 @@
+"""Calls of the rotation and paged-cache operators that their documentation allows: rows at any address.
+"""
+
+import pytest
+import torch
+
+from kiv_b200 import paged
+from kiv_b200.middleware import fused_rotary
+from tests.gpu_helpers import DEV
+from tests.test_gpu_paged import BF, FP, HF, Case
+
+pytestmark = pytest.mark.gpu
+
+
+def _shifted(x):
+    """The same values, contiguous, one element behind an aligned address."""
+    flat = torch.empty(x.numel() + 1, dtype=x.dtype, device=x.device)
+    y = flat[1:].view(x.shape)
+    y.copy_(x)
+    assert y.is_contiguous() and y.data_ptr() % 16
+    return y
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+def test_contiguous_rows_off_a_16_byte_boundary(dtype):
+    """Such rows are copied by the operators; results are those of aligned ones, to the bit."""
+    g = torch.Generator(device=DEV).manual_seed(1)
+    q, k = (torch.randn(2, h, 5, 64, generator=g, device=DEV).to(dtype) for h in (4, 2))
+    cos, sin = paged.rotary_table(1e4 ** (-torch.arange(32, dtype=torch.float64, device=DEV) / 32), 10)
+    w = torch.randn(64, generator=g, device=DEV).to(dtype)
+    want = paged.qk_norm_rope(q, k, cos, sin, eps=1e-6, q_weight=w, k_weight=w)
+    got = paged.qk_norm_rope(_shifted(q), _shifted(k), _shifted(cos), _shifted(sin), eps=1e-6, q_weight=_shifted(w), k_weight=_shifted(w))
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+    c = Case([3, 40], [30, 90], 8, 2, 64, 16, dtype)
+    want = paged.paged_attend(c.q, *c.args(), 0.1)
+    assert torch.equal(paged.paged_attend(_shifted(c.q), *c.args(), 0.1), want)
+    pages = [x.clone() for x in (c.kp, c.vp)]
+    paged.paged_append(c.k, c.v, *c.args(), cos=cos.repeat(9, 1), sin=sin.repeat(9, 1))
+    paged.paged_append(_shifted(c.k), _shifted(c.v), *pages, *c.args()[2:], cos=cos.repeat(9, 1), sin=sin.repeat(9, 1))
+    assert all(torch.equal(a.nan_to_num(7), b.nan_to_num(7)) for a, b in zip(pages, (c.kp, c.vp)))
+
+
+@torch.no_grad()
+def test_fused_rotation_of_rows_off_a_16_byte_boundary():
+    """Where the model's own function works, the one in its place does too."""
+    def fail(*args, **kwargs):
+        raise AssertionError("the kernel takes these")
+
+    q, k = torch.randn(1, 4, 3, 64, device=DEV, dtype=BF), torch.randn(1, 2, 3, 64, device=DEV, dtype=BF)
+    ang = torch.rand(1, 3, 32, device=DEV) * 6
+    cos, sin = (torch.cat([f, f], -1).to(BF) for f in (ang.cos(), ang.sin()))
+    turn = fused_rotary(fail)
+    want, got = turn(q, k, cos, sin), turn(_shifted(q), _shifted(k), _shifted(cos), _shifted(sin))
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
