@@ -148,11 +148,11 @@ def _repeats_halves(rotary: Any, device: torch.device) -> bool:
 def fused_rotary(original: Any):
     """``apply_rotary_pos_emb`` of a model as one kernel (``paged.qk_norm_rope``).
 
-    Inputs outside the kernel's -- CPU tensors, gradients, other layouts or
+    Inputs outside the kernel's -- CPU tensors, gradients and tangents, other layouts or
     dtypes, part of the head rotated -- go to the model's own function.  The
     kernel computes in float32 and rounds once, where the model's elementwise
     products round at each step."""
-    from .paged import qk_norm_rope
+    from .paged import needs_derivative, qk_norm_rope
 
     @functools.wraps(original)
     def apply_rotary_pos_emb(q, k, cos, sin, *args, **kwargs):
@@ -164,7 +164,7 @@ def fused_rotary(original: Any):
                  or q.dtype != k.dtype or q.dtype not in (torch.float32, torch.bfloat16, torch.float16)
                  or cos.dtype != sin.dtype or cos.dtype not in (q.dtype, torch.float32)
                  or (q.shape[-1] * q.element_size()) % 16 or q.shape[-1] * q.element_size() > 1024
-                 or (torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, cos, sin))))
+                 or needs_derivative(q, k, cos, sin))
         if plain:
             return original(q, k, cos, sin, *args, **kwargs)
         B, _, Q, D = q.shape

@@ -24,13 +24,15 @@ could not follow -- they never read or write out of bounds.
 
 Every call runs on the current stream of its tensors' device, allocates its
 scratch from that stream's pool and raises ``KIVNativeError`` on refused
-arguments.  There is no CPU implementation and no backward: inputs that require
-gradients are refused outside ``torch.no_grad()``.
+arguments.  There is no CPU implementation, no backward and no forward
+derivative: inputs that require gradients are refused outside
+``torch.no_grad()``, inputs with a forward-mode tangent everywhere.
 """
 
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as nat
 from . import ops
@@ -55,12 +57,20 @@ def _run(name: str, rows: torch.Tensor, *args) -> None:
         raise
 
 
+def needs_derivative(*tensors: torch.Tensor | None) -> bool:
+    """Whether a gradient or a forward-mode tangent of an input would have to come through the call."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return True
+    if getattr(forward_ad, "_current_level", 0) < 0:            # no dual level: spares the calls below
+        return False
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def _refuse_gradients(name: str, *tensors: torch.Tensor | None) -> None:
-    """There is no backward: an input that needs one is refused, its gradient would be missing without a word."""
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise nat.KIVNativeError(f"{name} has no backward: call it under torch.no_grad() or on detached tensors")
+    """There is no derivative: an input that needs one is refused, it would be missing without a word."""
+    if needs_derivative(*tensors):
+        raise nat.KIVNativeError(f"{name} has no backward and no forward derivative: call it under torch.no_grad(), on "
+                                 "detached tensors and on tensors without a tangent")
 
 
 def rotary_table(inv_freq: torch.Tensor, length: int, scaling: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:

@@ -53,3 +53,19 @@ def test_fused_rotation_of_rows_off_a_16_byte_boundary():
     turn = fused_rotary(fail)
     want, got = turn(q, k, cos, sin), turn(_shifted(q), _shifted(k), _shifted(cos), _shifted(sin))
     assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_fused_rotation_of_rows_with_a_tangent():
+    """The kernel has no derivative: the model's own function answers, tangent and all."""
+    def plain(q, k, cos, sin):
+        calls.append(1)
+        return q * cos[:, None], k * cos[:, None]
+
+    calls = []
+    turn = fused_rotary(plain)
+    q, k = torch.randn(1, 4, 3, 64, device=DEV), torch.randn(1, 2, 3, 64, device=DEV)
+    cos, sin = torch.rand(1, 3, 64, device=DEV), torch.rand(1, 3, 64, device=DEV)
+    got, tangent = torch.func.jvp(lambda x: turn(x, k, cos, sin)[0], (q,), (torch.ones_like(q),))
+    assert calls == [1] and torch.equal(got, q * cos[:, None]) and torch.equal(tangent, cos[:, None].expand_as(q))
+    turn(q, k, cos, sin)
+    assert calls == [1]
