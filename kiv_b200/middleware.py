@@ -20,6 +20,7 @@ import importlib
 import inspect
 import logging
 import sys
+import weakref
 from typing import Any
 
 import torch
@@ -173,6 +174,7 @@ def fused_rotary(original: Any):
         return qk_norm_rope(q, k, rows[0], rows[1])
 
     apply_rotary_pos_emb._kiv_original = original
+    apply_rotary_pos_emb._kiv_users = weakref.WeakSet()      # installed middlewares that asked for it
     return apply_rotary_pos_emb
 
 
@@ -195,7 +197,8 @@ class KIVMiddleware:
         """Route the model's global layers through KIV.  ``fused_rotary``: also
         turn queries and keys by one kernel in place of the model's elementwise
         rotation, for models whose rotation it is (half-split pairs); it stands
-        in the model's module, for every model of that family, until ``uninstall()``."""
+        in the model's module, for every model of that family, until the last
+        middleware that asked for it there is uninstalled."""
         if self._installed:
             logger.warning("KIV middleware already installed.")
             return
@@ -217,7 +220,9 @@ class KIVMiddleware:
                 ALL_MASK_ATTENTION_FUNCTIONS[self._original_impl])
         self._set_attn_impl(self._kiv_key)
         if fused_rotary:
-            self._fuse_rotary()
+            self._rotary_module = self._fuse_rotary()
+            if self._rotary_module is not None:
+                self._rotary_module.apply_rotary_pos_emb._kiv_users.add(self)
         self._installed = True
         logger.info("KIV middleware installed: %d global layers (%d independent, %d shared), "
                     "attn=%s, hot=%d, top_p=%d", len(self.topology.global_layer_indices),
@@ -232,7 +237,9 @@ class KIVMiddleware:
         if self._rotary_module is not None:
             fn = getattr(self._rotary_module, "apply_rotary_pos_emb", None)
             if hasattr(fn, "_kiv_original"):
-                self._rotary_module.apply_rotary_pos_emb = fn._kiv_original
+                fn._kiv_users.discard(self)
+                if not fn._kiv_users:
+                    self._rotary_module.apply_rotary_pos_emb = fn._kiv_original
             self._rotary_module = None
         if self._kiv_key is not None:
             if self._kiv_key in ALL_ATTENTION_FUNCTIONS:
@@ -322,7 +329,8 @@ class KIVMiddleware:
             raise RuntimeError("Call install() before chunked_retrieval_prefill().")
         return chunked_reuse_prefill(self.model, input_ids, cache, chunk_size=chunk_size)
 
-    def _fuse_rotary(self) -> None:
+    def _fuse_rotary(self) -> Any:
+        """The module in which the kernel stands in for the model's rotation, or None where it cannot."""
         attn = self._text_model.layers[self.topology.global_layer_indices[0]].self_attn
         module = sys.modules.get(type(attn).__module__)
         fn = getattr(module, "apply_rotary_pos_emb", None)
@@ -332,10 +340,10 @@ class KIVMiddleware:
                 or not _repeats_halves(rotary, device):
             logger.warning("fused_rotary: %s does not rotate half-split pairs through apply_rotary_pos_emb; left as it is",
                            type(attn).__name__)
-            return
+            return None
         if not hasattr(fn, "_kiv_original"):
             module.apply_rotary_pos_emb = fused_rotary(fn)
-            self._rotary_module = module
+        return module
 
     def _resolve_attn_impl(self) -> str:
         cfg = self.model.config

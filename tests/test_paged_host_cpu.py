@@ -28,3 +28,45 @@ def test_inputs_with_a_tangent_are_refused():
                 call(lambda x: x)
     with pytest.raises(nat.KIVNativeError, match="tangent"):
         torch.func.jvp(lambda x: paged.qk_norm_rope(x, None, eps=1e-6)[0], (q,), (q,))
+
+
+def _llama():
+    from transformers import LlamaConfig, LlamaForCausalLM
+    return LlamaForCausalLM(LlamaConfig(vocab_size=64, hidden_size=64, intermediate_size=64, num_hidden_layers=1,
+                                        num_attention_heads=2, num_key_value_heads=1, head_dim=32,
+                                        attn_implementation="eager")).eval()
+
+
+@pytest.mark.parametrize("first", [0, 1])
+def test_fused_rotation_stays_until_the_last_model_leaves(first):
+    """Two models of one family ask for the kernel: the one that leaves first does not take it from the other."""
+    import sys
+    from kiv_b200 import KIVConfig, KIVMiddleware
+
+    users = [KIVMiddleware(_llama(), KIVConfig()) for _ in range(2)]
+    module = sys.modules[type(users[0].model.model.layers[0].self_attn).__module__]
+    before = module.apply_rotary_pos_emb
+    for _ in range(2):                                      # and again after both have left
+        for mw in users:
+            mw.install(fused_rotary=True)
+        fused = module.apply_rotary_pos_emb
+        assert fused._kiv_original is before                # not stacked
+        users[first].uninstall()
+        assert module.apply_rotary_pos_emb is fused
+        users[1 - first].uninstall()
+        assert module.apply_rotary_pos_emb is before
+
+
+def test_a_model_without_the_fused_rotation_does_not_hold_it():
+    import sys
+    from kiv_b200 import KIVConfig, KIVMiddleware
+
+    asks, does_not = (KIVMiddleware(_llama(), KIVConfig()) for _ in range(2))
+    module = sys.modules[type(asks.model.model.layers[0].self_attn).__module__]
+    before = module.apply_rotary_pos_emb
+    asks.install(fused_rotary=True)
+    does_not.install()
+    asks.uninstall()
+    assert module.apply_rotary_pos_emb is before
+    does_not.uninstall()
+    assert module.apply_rotary_pos_emb is before
