@@ -150,7 +150,7 @@ def fused_rotary(original: Any):
     """``apply_rotary_pos_emb`` of a model as one kernel (``paged.qk_norm_rope``).
 
     Inputs outside the kernel's -- CPU tensors, gradients and tangents, other layouts or
-    dtypes, part of the head rotated -- go to the model's own function.  The
+    mixed dtypes, part of the head rotated -- go to the model's own function.  The
     kernel computes in float32 and rounds once, where the model's elementwise
     products round at each step."""
     from .paged import needs_derivative, qk_norm_rope
@@ -161,9 +161,10 @@ def fused_rotary(original: Any):
                  or any(n != "unsqueeze_dim" for n in kwargs)
                  or not (q.is_cuda and k.is_cuda and cos.is_cuda and sin.is_cuda)
                  or q.dim() != 4 or k.dim() != 4 or cos.dim() != 3 or cos.shape != sin.shape
+                 or k.shape[0] != q.shape[0] or k.shape[2:] != q.shape[2:] or cos.stride() != sin.stride() or cos.stride(-1) != 1
                  or cos.shape[-1] != q.shape[-1] or cos.shape[1] != q.shape[2] or cos.shape[0] not in (1, q.shape[0])
                  or q.dtype != k.dtype or q.dtype not in (torch.float32, torch.bfloat16, torch.float16)
-                 or cos.dtype != sin.dtype or cos.dtype not in (q.dtype, torch.float32)
+                 or cos.dtype != q.dtype or sin.dtype != q.dtype       # else the model's products have a wider dtype
                  or (q.shape[-1] * q.element_size()) % 16 or q.shape[-1] * q.element_size() > 1024
                  or needs_derivative(q, k, cos, sin))
         if plain:

@@ -70,3 +70,35 @@ def test_a_model_without_the_fused_rotation_does_not_hold_it():
     assert module.apply_rotary_pos_emb is before
     does_not.uninstall()
     assert module.apply_rotary_pos_emb is before
+
+
+@torch.no_grad()
+def test_fused_rotation_leaves_what_the_kernel_would_answer_otherwise():
+    """Mixed dtypes (the model's products are then in the wider one), and shapes and layouts that only broadcasting takes."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from kiv_b200 import ops
+    from kiv_b200.middleware import fused_rotary
+
+    ops.load()
+    calls = []
+
+    def plain(q, k, cos, sin):
+        calls.append(1)
+        c, s = cos[:, None], sin[:, None]
+        half = q.shape[-1] // 2
+        return tuple(x * c + torch.cat([-x[..., half:], x[..., :half]], -1) * s for x in (q, k))
+
+    turn = fused_rotary(plain)
+    with FakeTensorMode():
+        def t(*shape, dtype=torch.bfloat16):
+            return torch.empty(shape, dtype=dtype, device="cuda")
+
+        q, k, cs = t(2, 4, 3, 64), t(2, 2, 3, 64), t(2, 3, 64)
+        f32 = t(2, 3, 64, dtype=torch.float32)
+        for args, taken in [((q, k, cs, cs), True), ((q, k, cs[:1], cs[:1]), True), ((q, k, f32, f32), False),
+                            ((q, k, cs, f32), False), ((q, t(2, 2, 1, 64), cs, cs), False), ((q, t(1, 2, 3, 64), cs, cs), False),
+                            ((q, k, cs, t(3, 2, 64).transpose(0, 1)), False), ((q, k, *[t(2, 64, 3).mT] * 2), False)]:
+            calls.clear()
+            got, want = turn(*args), plain(*args)
+            assert len(calls) == (1 if taken else 2)
+            assert [(x.dtype, x.shape) for x in got] == [(x.dtype, x.shape) for x in want]
