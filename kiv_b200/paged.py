@@ -31,6 +31,8 @@ derivative: inputs that require gradients are refused outside
 
 from __future__ import annotations
 
+from array import array
+
 import torch
 from torch.autograd import forward_ad
 
@@ -144,6 +146,59 @@ def paged_attend(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
     return (out, lse) if return_lse else out
 
 
+class _PageBook:
+    """Which pages each sequence holds, and which cells of the block table a step changes (host only).
+
+    Slot i of the table remembers whose row it holds and how much of it is written: while a sequence keeps its slot, a step
+    costs the pages that are new, whatever it holds already.
+    """
+
+    def __init__(self, num_pages: int, page_size: int, max_batch: int, width: int) -> None:
+        self.page_size, self.max_batch, self.width = page_size, max_batch, width
+        self.unused = list(range(num_pages - 1, -1, -1))
+        self.held: dict = {}
+        self.lengths: dict = {}
+        self._slots: list = [(None, 0)] * max_batch             # (a sequence's list of pages, entries written)
+
+    def step(self, new: list[tuple]) -> tuple[list[int], list[int], list[tuple], array]:
+        """Row starts, lengths, and the changed cells: runs (first, count) of ``[max_batch, width]`` laid flat, and the pages
+        of all of them."""
+        if len(new) > self.max_batch:
+            raise ValueError(f"{len(new)} sequences exceed max_batch {self.max_batch}")
+        if len({s for s, _ in new}) != len(new):
+            raise ValueError("a sequence appears twice in one step")
+        need = []
+        for seq, n in new:
+            if n < 0:
+                raise ValueError("negative token count")
+            pages = -(-(self.lengths.get(seq, 0) + n) // self.page_size)
+            if pages > self.width:
+                raise nat.KIVNativeError(f"sequence {seq!r} needs {pages} pages, a sequence holds at most {self.width}")
+            need.append(pages - len(self.held.get(seq, ())))
+        if sum(need) > len(self.unused):
+            raise nat.KIVNativeError(f"out of pages: the step needs {sum(need)}, {len(self.unused)} are free")
+        starts, lens, runs, pages = [0], [], [], array("i")
+        for i, (seq, n) in enumerate(new):
+            held = self.held.setdefault(seq, array("i"))
+            held.extend(self.unused.pop() for _ in range(need[i]))
+            self.lengths[seq] = self.lengths.get(seq, 0) + n
+            lens.append(self.lengths[seq])
+            starts.append(starts[-1] + n)
+            owner, written = self._slots[i]
+            keep = written if owner is held else 0
+            end = max(written, len(held))                       # a longer row before it: no page from there on
+            if keep < end:
+                runs.append((i * self.width + keep, end - keep))
+                pages.extend(held[keep:])
+                pages.extend([-1] * (end - len(held)))
+                self._slots[i] = (held, len(held))
+        return starts, lens, runs, pages
+
+    def free(self, seq) -> None:
+        self.unused.extend(reversed(self.held.pop(seq, ())))
+        self.lengths.pop(seq, None)
+
+
 class PagedKVCache:
     """Pages of a model's KV layers for a batch of sequences of unequal lengths.
 
@@ -181,53 +236,27 @@ class PagedKVCache:
         self._lens = torch.zeros(max_batch, dtype=torch.int32, device=device)
         self._starts = torch.zeros(max_batch + 1, dtype=torch.int32, device=device)
         self.errors = torch.zeros(1, dtype=torch.int64, device=device)
-        self._rows = torch.full((max_batch, width), -1, dtype=torch.int32)     # host copy of the table
-        self._free = list(range(num_pages - 1, -1, -1))
-        self._pages: dict = {}
-        self._length: dict = {}
+        self._book = _PageBook(num_pages, page_size, max_batch, width)
         self._batch = self._tokens = self._most = 0
 
     # ------------------------------------------------------------------ host
     @property
     def free_pages(self) -> int:
-        return len(self._free)
+        return len(self._book.unused)
 
     def length(self, seq) -> int:
         """Tokens of a sequence, those of the current step included (0: unknown)."""
-        return self._length.get(seq, 0)
+        return self._book.lengths.get(seq, 0)
 
     def step(self, new: list[tuple]) -> int:
         """Begin a step: ``new`` lists ``(sequence, new tokens)`` in the order of the packed rows; unknown sequences
-        start empty.  Reserves their pages and uploads table, lengths and row starts.  Returns the number of rows."""
-        if len(new) > self.max_batch:
-            raise ValueError(f"{len(new)} sequences exceed max_batch {self.max_batch}")
-        if len({s for s, _ in new}) != len(new):
-            raise ValueError("a sequence appears twice in one step")
-        need = {}
-        for seq, n in new:
-            if n < 0:
-                raise ValueError("negative token count")
-            pages = -(-(self.length(seq) + n) // self.page_size)
-            if pages > self._table.shape[1]:
-                raise nat.KIVNativeError(f"sequence {seq!r} needs {pages} pages, a sequence holds at most {self._table.shape[1]}")
-            need[seq] = pages - len(self._pages.get(seq, ()))
-        if sum(need.values()) > len(self._free):
-            raise nat.KIVNativeError(f"out of pages: the step needs {sum(need.values())}, {len(self._free)} are free")
-        starts, lens = [0], []
-        rows = self._rows[:len(new)].clone()
-        for i, (seq, n) in enumerate(new):
-            held = self._pages.setdefault(seq, [])
-            held.extend(self._free.pop() for _ in range(need[seq]))
-            self._length[seq] = self.length(seq) + n
-            lens.append(self._length[seq])
-            starts.append(starts[-1] + n)
-            rows[i, :len(held)] = torch.tensor(held, dtype=torch.int32)
-            rows[i, len(held):] = -1
-        changed = (rows != self._rows[:len(new)]).any(1).nonzero().flatten().tolist()
-        self._rows[:len(new)] = rows
-        if changed:
-            lo, hi = changed[0], changed[-1] + 1
-            self._upload(self._table[lo:hi], rows[lo:hi])
+        start empty.  Reserves their pages and uploads lengths, row starts and what changed of the table: host work per
+        sequence and new page, not per page held.  Returns the number of rows."""
+        starts, lens, runs, pages = self._book.step(new)
+        if runs:
+            page = torch.frombuffer(pages, dtype=torch.int32)
+            at = torch.cat([torch.arange(first, first + count) for first, count in runs])
+            self._table.view(-1).index_copy_(0, *(x.pin_memory().to(self.device, non_blocking=True) for x in (at, page)))
         self._upload(self._lens[:len(new)], torch.tensor(lens, dtype=torch.int32))
         self._upload(self._starts[:len(new) + 1], torch.tensor(starts, dtype=torch.int32))
         self._batch, self._tokens, self._most = len(new), starts[-1], max([n for _, n in new], default=0)
@@ -239,8 +268,7 @@ class PagedKVCache:
 
     def free(self, seq) -> None:
         """Give a sequence's pages back (a step that is still running may read them: free after it)."""
-        self._free.extend(reversed(self._pages.pop(seq, [])))
-        self._length.pop(seq, None)
+        self._book.free(seq)
 
     # ---------------------------------------------------------------- device
     def arrays(self) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:

@@ -1,10 +1,10 @@
-"""Calls of the rotation and paged-cache operators that their documentation allows: rows at any address.
-"""
+"""Calls of the rotation and paged-cache operators that their documentation allows: rows at any address, steps of a cache
+whose sequences come and go, capture before the first token."""
 
 import pytest
 import torch
 
-from kiv_b200 import paged
+from kiv_b200 import PagedKVCache, paged
 from kiv_b200.middleware import fused_rotary
 from tests.gpu_helpers import DEV
 from tests.test_gpu_paged import BF, FP, HF, Case
@@ -69,3 +69,27 @@ def test_fused_rotation_of_rows_with_a_tangent():
     assert calls == [1] and torch.equal(got, q * cos[:, None]) and torch.equal(tangent, cos[:, None].expand_as(q))
     turn(q, k, cos, sin)
     assert calls == [1]
+
+
+def test_the_table_of_a_cache_follows_its_sequences():
+    """Sequences that come, go, change places and take an old name: the device table is each step's sequences' pages, and a
+    step waits for nothing on the device."""
+    cache = PagedKVCache(40, 4, 1, 64, device=DEV, max_batch=4, max_pages_per_seq=9)
+    steps = [[("a", 9), ("b", 30)], [("a", 1), ("b", 1)], [("b", 1), ("a", 3)], "b", [("c", 5), ("a", 1), ("b", 2)], [("a", 1)], "a",
+             [("a", 4), ("d", 36), ("c", 0), ("b", 3)], [("a", 1), ("c", 8), ("b", 1)], "d", [("c", 1), ("d", 1)]]
+    for new in steps:
+        if isinstance(new, str):
+            cache.free(new)
+            continue
+        torch.cuda.set_sync_debug_mode("error")
+        try:
+            rows = cache.step(new)
+        finally:
+            torch.cuda.set_sync_debug_mode("default")
+        table, lens, starts = (x.tolist() for x in cache.arrays())
+        assert rows == starts[-1] and lens == [cache.length(s) for s, _ in new]
+        seen = set()
+        for row, n, (s, _) in zip(table, lens, new):
+            held = -(-n // 4)
+            assert all(p >= 0 for p in row[:held]) and row[held:] == [-1] * (9 - held) and not seen & set(row[:held])
+            seen |= set(row[:held])

@@ -102,3 +102,74 @@ def test_fused_rotation_leaves_what_the_kernel_would_answer_otherwise():
             got, want = turn(*args), plain(*args)
             assert len(calls) == (1 if taken else 2)
             assert [(x.dtype, x.shape) for x in got] == [(x.dtype, x.shape) for x in want]
+
+
+def _random_steps(rng, book, names, pages):
+    """A step's list: some of the sequences in any order, with tokens that fit."""
+    some = rng.sample(names, rng.randint(1, min(len(names), book.max_batch)))
+    free, out = len(book.unused), []
+    for s in some:
+        n = rng.choice([0, 1, 1, 5, 3 * book.page_size])
+        have = book.lengths.get(s, 0)
+        need = -(-(have + n) // book.page_size) - len(book.held.get(s, ()))
+        if need <= free and -(-(have + n) // book.page_size) <= pages:
+            free -= need
+            out.append((s, n))
+    return out
+
+
+def test_the_changed_cells_make_the_block_table():
+    """Steps of random sequences in random order, some given back, some under an old name: the cells applied one step after
+    the other give each row its sequence's pages and -1 behind them, and no page has two owners."""
+    import random
+
+    rng = random.Random(5)
+    book = paged._PageBook(40, 4, 5, 12)
+    table = [-1] * (5 * 12)
+    names = list("abcdefg")
+    for _ in range(400):
+        new = _random_steps(rng, book, names, 12)
+        starts, lens, runs, pages = book.step(new)
+        cells = [at for first, count in runs for at in range(first, first + count)]
+        assert len(set(cells)) == len(cells) == len(pages)
+        for at, page in zip(cells, pages):
+            table[at] = page
+        for i, (s, n) in enumerate(new):
+            held = list(book.held[s])
+            assert len(held) == -(-lens[i] // 4) and starts[i + 1] - starts[i] == n and lens[i] == book.lengths[s]
+            assert table[i * 12:i * 12 + 12] == held + [-1] * (12 - len(held))
+        owned = [p for held in book.held.values() for p in held]
+        assert sorted(owned + book.unused) == list(range(40))
+        if rng.random() < 0.3:
+            book.free(rng.choice(names))
+
+
+def test_a_decode_step_costs_the_new_pages_not_the_held_ones():
+    """64 sequences of 2048 pages: a token each changes a cell where a page begins, none elsewhere, and takes no longer
+    than with one page per sequence (a step that walked every page held would take hundreds of times as long)."""
+    import time
+
+    def decode(held):
+        book = paged._PageBook(64 * (held + 8), 16, 64, 64 * (held + 8))
+        step = [(s, 1) for s in range(64)]
+        book.step([(s, 16 * (held - 1) + s % 16) for s in range(64)])
+        took = []
+        for _ in range(64):
+            t = time.perf_counter()
+            _, lens, _, pages = book.step(step)
+            took.append(time.perf_counter() - t)
+            assert len(pages) == sum((n - 1) % 16 == 0 for n in lens)
+        return min(took)
+
+    decode(1)
+    assert decode(2048) < 10 * decode(1)
+
+
+def test_a_step_that_does_not_fit_changes_nothing_of_the_book():
+    book = paged._PageBook(4, 8, 2, 3)
+    book.step([("a", 10)])
+    for new, error in [([("a", 7), ("b", 16)], nat.KIVNativeError), ([("a", 20)], nat.KIVNativeError),
+                       ([("a", 1), ("a", 1)], ValueError), ([("b", -1)], ValueError), ([(s, 0) for s in "abc"], ValueError)]:
+        with pytest.raises(error):
+            book.step(new)
+        assert book.lengths == {"a": 10} and list(book.held) == ["a"] and len(book.unused) == 2
