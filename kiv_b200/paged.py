@@ -213,7 +213,11 @@ class PagedKVCache:
     ``step`` is host work (it raises before it changes anything when the pages
     run out); ``append`` and ``attend`` read its device arrays, which stay where
     they are, so a captured ``append`` / ``attend`` serves later steps of the
-    same batch size and token count.  ``errors`` collects the kernels' bits.
+    same number of sequences and at most the captured number of rows.  To
+    capture before their tokens are there, begin a step of the sequences with 0
+    new tokens each and pass rows of the later number: nothing is written while
+    capturing, and the replay after the next ``step`` finds its tokens.
+    ``errors`` collects the kernels' bits.
     """
 
     def __init__(self, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int, *, layers: int = 1,

@@ -93,3 +93,36 @@ def test_the_table_of_a_cache_follows_its_sequences():
             held = -(-n // 4)
             assert all(p >= 0 for p in row[:held]) and row[held:] == [-1] * (9 - held) and not seen & set(row[:held])
             seen |= set(row[:held])
+
+
+@pytest.mark.parametrize("D,S", [(128, 16), (80, 10)])
+def test_capture_before_the_first_token_and_steps_of_fewer_rows(D, S):
+    """A layer captured over a step without tokens serves steps of up to the captured rows; the rows of the captured call
+    behind a step's tokens stay as they are."""
+    caches = [PagedKVCache(64, S, 2, D, dtype=BF, device=DEV, max_batch=3) for _ in range(2)]
+    g = torch.Generator(device=DEV).manual_seed(2)
+    q, k, v = (torch.zeros(6, h, D, device=DEV, dtype=BF) for h in (8, 2, 2))
+    out = torch.zeros_like(q)
+    caches[0].step([(s, 0) for s in "xyz"])
+    before = caches[0].k.clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        caches[0].append(0, k, v)
+        caches[0].attend(0, q, 0.1, out=out)
+    assert torch.equal(caches[0].k, before)
+    for new in ([2, 1, 3], [1, 1, 1], [0, 5, 0], [2, 2, 2], [1, 0, 1]):
+        for t in (q, k, v):
+            t.normal_(generator=g)
+        out.fill_(7)
+        rows = [c.step(list(zip("xyz", new))) for c in caches]
+        assert rows == [sum(new)] * 2
+        graph.replay()
+        caches[1].append(0, k[:rows[0]], v[:rows[0]])
+        want = caches[1].attend(0, q[:rows[0]], 0.1)
+        if D == 128:
+            assert torch.equal(out[:rows[0]], want)
+        else:       # other row counts, other order of sums: each within half a step and 2e-5 of the values' largest
+            assert ((out[:rows[0]] - want).abs() <= 2.0 ** -7 * want.abs() + 4e-5 * 6).all()
+        assert (out[rows[0]:] == 7).all() and torch.equal(*[c.k for c in caches])
+    assert int(caches[0].errors) == 0
