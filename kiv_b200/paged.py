@@ -61,11 +61,15 @@ def _run(name: str, rows: torch.Tensor, *args) -> None:
 
 def needs_derivative(*tensors: torch.Tensor | None) -> bool:
     """Whether a gradient or a forward-mode tangent of an input would have to come through the call."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        return True
-    if getattr(forward_ad, "_current_level", 0) < 0:            # no dual level: spares the calls below
-        return False
-    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    if getattr(forward_ad, "_current_level", 0) >= 0:           # inside a dual level, where there can be tangents
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                return True
+    return False
 
 
 def _refuse_gradients(name: str, *tensors: torch.Tensor | None) -> None:
