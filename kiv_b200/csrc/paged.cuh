@@ -20,6 +20,14 @@ __device__ __forceinline__ void paged_error(int64_t *errors, int64_t bit) {
   if (errors) atomicOr(reinterpret_cast<unsigned long long *>(errors), (unsigned long long)bit);
 }
 
+// After a wait that ran out, copies may still be on the way to the block's shared
+// memory, in phases of their barriers that nobody counted: holds the block for as
+// long as the wait itself was given (2^31 cycles).
+__device__ __forceinline__ void paged_linger() {
+  const long long t0 = clock64();
+  while (clock64() - t0 < (1ll << 31)) __nanosleep(1000);
+}
+
 // One sequence: its new tokens' first packed row and count, and its length.
 // Lengths and row ranges are clamped to what the arrays hold, so nothing a
 // device array says can lead out of bounds.

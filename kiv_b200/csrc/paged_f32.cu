@@ -357,7 +357,10 @@ __global__ void __launch_bounds__(MF_THREADS, F32Shape<D, 16 * WM>::BLOCKS) page
     }
     paged_advance(p, at, sg);
   }
-  if (!ok) paged_error(p.pc.errors, KIV_ERRBIT_WAIT_TIMEOUT);
+  if (!ok) {
+    paged_error(p.pc.errors, KIV_ERRBIT_WAIT_TIMEOUT);
+    paged_linger();
+  }
 }
 
 // ------------------------------------------------------------------ host

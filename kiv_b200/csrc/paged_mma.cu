@@ -383,7 +383,10 @@ __global__ void __launch_bounds__(MM_THREADS, MmaShape<D, 16 * WM>::BLOCKS) page
     }
     paged_advance(p, at, sg);
   }
-  if (!ok) paged_error(p.pc.errors, KIV_ERRBIT_WAIT_TIMEOUT);
+  if (!ok) {
+    paged_error(p.pc.errors, KIV_ERRBIT_WAIT_TIMEOUT);
+    paged_linger();
+  }
 }
 
 // ------------------------------------------------------------------ host

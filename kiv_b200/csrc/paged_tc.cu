@@ -66,7 +66,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
   using T = typename std::conditional<BF, __nv_bfloat16, __half>::type;
   constexpr int SLOTS = S::SLOTS;
   extern __shared__ uint8_t pt_dyn[];
-  __shared__ uint64_t q_full, q_empty, kv_full[SLOTS], kv_empty[SLOTS], s_full[2], p_full[2], p_tail[2], o_full[2];
+  __shared__ uint64_t q_full, q_empty, kv_full[SLOTS], kv_empty[SLOTS], s_full[2], p_full[2], p_tail[2], o_full[2], halt[2];
   __shared__ uint32_t s_tmem;
   __shared__ PtSeg seg[2];
   __shared__ float s_ml[2][PT_ROWS];           // of the second of two twins
@@ -87,6 +87,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
       mbar_init(&p_full[i], 4);
       mbar_init(&p_tail[i], 4);
       mbar_init(&o_full[i], 1);
+      mbar_init(&halt[i], 1);
     }
     mbar_fence_init();
   }
@@ -107,7 +108,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
   tc::fence_after_sync();
   const uint32_t tmem = s_tmem;
   griddep_wait();
-  bool ok = true;
+  bool ok = true, mma = false;
+  uint32_t turn = 0, qturn = 0;                // what this warp asked TMA for
   const int rows = g.tps * p.grp;              // of a row tile
   if (warp >= 8) {
    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PT_REGS_OTHER));
@@ -143,7 +145,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
         if (told) return;
         if (items > 0 && !must && !__shfl_sync(KIV_FULL_MASK, (int)mbar_test(&q_empty, (items - 1) & 1), 0)) return;
         if (items > 0 && ok && !mbar_wait_bounded(&q_empty, (items - 1) & 1)) ok = false;
-        if (lane == 0) {
+        if (lane == 0 && ok) {
           seg[items & 1] = sg;
           if (ntile == 0) {
             mbar_arrive(&q_full);
@@ -169,7 +171,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
           tell(2 * t + kv >= SLOTS);           // from there on a slot waits for this item's own tiles
           const uint32_t s = n % SLOTS;
           if (n >= SLOTS && ok && !mbar_wait_bounded(&kv_empty[s], (n / SLOTS - 1) & 1)) ok = false;
-          __syncwarp();
+          if (!__all_sync(KIV_FULL_MASK, ok)) goto halted;     // nothing more is asked for
           if (me == 0 && leader) mbar_arrive_tx(&kv_full[s], S::TILE);
           const CUtensorMap *map = kv ? &vmap : &kmap;
           for (int x = me; x < nbox * S::NB; x += 2) {      // box x / NB, columns x % NB
@@ -187,6 +189,9 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
       }
       paged_advance(p, at, cut);
     }
+   halted:
+    turn = n;
+    qturn = items + 1;                         // a query tile not asked for: its wait ends at the limit
    } else if (warp < 11) {
     // ------------------------------------------------ MMA of row tile i
     // The tensor pipe takes few products ahead, so what an issuing warp does
@@ -204,6 +209,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
     uint32_t slot = 0, phase = 0;              // of the next K or V tile
     uint32_t tiles = 0;
     const bool leader = elect_one();
+    mma = leader;
     auto wait = [&](uint64_t *bar, uint32_t parity) {
       if (ok && !mbar_wait_bounded(bar, parity)) ok = false;
     };
@@ -518,7 +524,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant_
   }
   if (!ok) paged_error(p.pc.errors, KIV_ERRBIT_WAIT_TIMEOUT);
   tc::fence_before_sync();
-  __syncthreads();
+  pt_finish<SLOTS>(ok, kv_full, turn, &q_full, qturn, mma, &halt[warp == 10]);
   tc::fence_after_sync();
   if (warp == 9) tc::tmem_dealloc(tmem, 512);
 }

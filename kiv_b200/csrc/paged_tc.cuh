@@ -150,6 +150,33 @@ __device__ __forceinline__ float pt_reference(float m, float c) {
   return (BF ? m * c : m * c - PT_BIAS<BF>) * 0.693147181f;
 }
 
+// Waits, with a limit, for the copies that are on the way to a ring of N stages
+// whose next turn is `turn`.
+template <int N>
+__device__ __forceinline__ void pt_drain(uint64_t *full, uint32_t turn) {
+#pragma unroll 1
+  for (uint32_t k = 1; k <= N && k <= turn; ++k)
+    if (!mbar_wait_bounded(&full[(turn - k) % N], ((turn - k) / N) & 1)) return;
+}
+
+// Where a wait ran out, a role goes on without its waits or leaves, so copies and
+// products on the way may outlast the roles.  End of the kernel, all threads:
+// waits for them, again with a limit, before the block's memory is given back.
+// turn, qturn: the ring's turns and the query tiles that this lane's warp asked
+// TMA for; mma: the lane of an MMA warp that issued its products.
+template <int SLOTS>
+__device__ __forceinline__ void pt_finish(bool ok, uint64_t *kv_full, uint32_t turn, uint64_t *q_full, uint32_t qturn, bool mma,
+                                          uint64_t *halt) {
+  if (__syncthreads_or(ok ? 0 : 1) == 0) return;
+  if (qturn > 0) mbar_wait_bounded(q_full, (qturn - 1) & 1);
+  pt_drain<SLOTS>(kv_full, turn);
+  if (mma) {
+    tc::commit(halt);
+    mbar_wait_bounded(halt, 0);
+  }
+  __syncthreads();
+}
+
 // One segment of the block's stretch, as the TMA warp tells the others.
 struct PtSeg {
   int ntile;       // 0: no more

@@ -44,7 +44,7 @@ paged_tc256_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
                    const __grid_constant__ CUtensorMap vmap, const __grid_constant__ PagedPlan p, PagedTcGeom g) {
   using T = typename std::conditional<BF, __nv_bfloat16, __half>::type;
   extern __shared__ __align__(1024) uint8_t p2_dyn[];
-  __shared__ uint64_t q_full, q_empty, kv_full[P2_SLOTS], kv_empty[P2_SLOTS], s_full[2], p_full[2], pv_done[2];
+  __shared__ uint64_t q_full, q_empty, kv_full[P2_SLOTS], kv_empty[P2_SLOTS], s_full[2], p_full[2], pv_done[2], halt[2];
   __shared__ uint32_t s_tmem;
   __shared__ PtSeg seg[2];
   const int warp = __shfl_sync(KIV_FULL_MASK, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
@@ -62,6 +62,7 @@ paged_tc256_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 8);
       mbar_init(&pv_done[i], 1);
+      mbar_init(&halt[i], 1);
     }
     mbar_fence_init();
   }
@@ -82,7 +83,8 @@ paged_tc256_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
   tc::fence_after_sync();
   const uint32_t tmem = s_tmem;                // scores [0, 256), output [256, 512)
   griddep_wait();
-  bool ok = true;
+  bool ok = true, mma = false;
+  uint32_t turn = 0, qturn = 0;                // what this warp asked TMA for
   auto wait = [&](uint64_t *bar, uint32_t parity) {
     if (ok && !mbar_wait_bounded(bar, parity)) ok = false;
   };
@@ -98,7 +100,8 @@ paged_tc256_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
     P2Ring r;
     const int nbox = PT_KEYS / g.br, half = 64 / g.br;    // boxes of a K tile; of a V half
     if (me == 0 && lane == 0) p.cut[blockIdx.x].b = -1;
-    for (uint32_t items = 0;; ++items) {
+    uint32_t items = 0;
+    for (;; ++items) {
       PtSeg sg = {};
       PagedSegment cut = {};
       int kvh = 0;
@@ -120,7 +123,7 @@ paged_tc256_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         if (told) return;
         if (items > 0 && !must && !__shfl_sync(KIV_FULL_MASK, (int)mbar_test(&q_empty, (items - 1) & 1), 0)) return;
         if (items > 0) wait(&q_empty, (items - 1) & 1);
-        if (lane == 0) {
+        if (lane == 0 && ok) {
           seg[items & 1] = sg;
           if (ntile == 0) {
             mbar_arrive(&q_full);
@@ -137,16 +140,20 @@ paged_tc256_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         tell(true);
         break;
       }
-      auto begin = [&](uint32_t h) {
+      auto begin = [&](uint32_t h) {           // nullptr: a wait ran out, nothing more is asked for
         tell(slots++ >= P2_SLOTS);
         if (r.n + h >= P2_SLOTS) wait(&kv_empty[r.slot(h)], r.parity(h) ^ 1);
-        __syncwarp();
+        if (!__all_sync(KIV_FULL_MASK, ok)) {
+          turn = turn > 0 ? turn : r.n + h;
+          return (uint8_t *)nullptr;
+        }
         if (me == 0 && leader) mbar_arrive_tx(&kv_full[r.slot(h)], P2_SLOT);
         return ring + r.slot(h) * P2_SLOT;
       };
       auto load_k = [&](int32_t page, int32_t row) {   // slot h: columns [128 h, 128 h + 128) of all rows
         for (uint32_t h = 0; h < 2; ++h) {
           uint8_t *dst = begin(h);
+          if (!dst) break;
           for (int l = 0; l < nbox; ++l) {
             const int32_t bp = __shfl_sync(KIV_FULL_MASK, page, l), br = __shfl_sync(KIV_FULL_MASK, row, l);
             if (leader) tc::tma_load_4d(dst + me * (PT_KEYS * 128) + l * g.br * 128, &kmap, (2 * h + me) * 64, br, kvh, bp, &kv_full[r.slot(h)]);
@@ -157,6 +164,7 @@ paged_tc256_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
       auto load_v = [&](int32_t page, int32_t row) {   // slot h: rows [64 h, 64 h + 64)
         for (uint32_t h = 0; h < 2; ++h) {
           uint8_t *dst = begin(h);
+          if (!dst) break;
           for (int l = 0; l < half; ++l) {
             const int32_t bp = __shfl_sync(KIV_FULL_MASK, page, h * half + l), br = __shfl_sync(KIV_FULL_MASK, row, h * half + l);
             if (leader) {
@@ -185,13 +193,17 @@ paged_tc256_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         if (!cut.head) paged_check_lens(p.pc, at.it.s);
         if (cut.tail) paged_record(p, blockIdx.x, at, cut);
       }
+      if (!__all_sync(KIV_FULL_MASK, ok)) break;
       paged_advance(p, at, cut);
     }
+    if (__all_sync(KIV_FULL_MASK, ok)) turn = r.n;
+    qturn = items + 1;                         // a query tile not asked for: its wait ends at the limit
    } else if (warp == 9) {
     // ------------------------------------------------ S = Q K^T
     constexpr uint32_t id_s = tc::idesc_f16(BF, PT_ROWS, PT_KEYS);
     const uint64_t qd = tc::sdesc_k128(smem_u32(qmem)), kd = tc::sdesc_k128(smem_u32(ring));
     const bool leader = elect_one();
+    mma = leader;
     P2Ring r;
     uint32_t tiles = 0;
     for (uint32_t items = 0;; ++items) {
@@ -228,6 +240,7 @@ paged_tc256_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
     constexpr uint32_t id_o = tc::idesc_f16(BF, PT_ROWS, P2_D) | (1u << 16);   // B is MN-major
     const uint64_t vd = tc::sdesc_mn<128>(smem_u32(ring), 64 * 128);
     const bool leader = elect_one();
+    mma = leader;
     P2Ring r;
     uint32_t tiles = 0;
     for (uint32_t items = 0;; ++items) {
@@ -450,7 +463,7 @@ paged_tc256_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
   }
   if (!ok) paged_error(p.pc.errors, KIV_ERRBIT_WAIT_TIMEOUT);
   tc::fence_before_sync();
-  __syncthreads();
+  pt_finish<P2_SLOTS>(ok, kv_full, turn, &q_full, qturn, mma, &halt[warp == 10]);
   tc::fence_after_sync();
   if (warp == 9) tc::tmem_dealloc(tmem, 512);
 }
