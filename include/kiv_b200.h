@@ -427,7 +427,7 @@ typedef struct kiv_paged {
   int64_t table_stride, table_width;
   const int32_t *seq_lens, *q_starts;
   int64_t num_tokens;
-  int64_t *errors;          /* device word that collects KIV_ERRBIT_* (never cleared here), or NULL */
+  int64_t *errors;          /* device word that collects KIV_ERRBIT_* (never cleared here), or NULL: they are lost */
 } kiv_paged;
 
 /* Norm and rotation of rows: y = x * rsqrt(mean(x^2) + eps) * (weight_offset +
@@ -500,8 +500,17 @@ typedef struct kiv_paged_query {
  * the natural logarithm of the sum of exp(score).  A row that sees no key gets
  * out 0 and lse -inf.  Keys whose page number is outside [0, num_pages) read as
  * rows of zeros.  Rows of the pages past a sequence's length, and of pages no
- * row of a tile sees, never reach a result, whatever they hold.
+ * row of a tile sees, never reach a result, whatever they hold; a NaN or an
+ * infinity in the value row of a live key reaches the rows of its tile that do
+ * not see the key, too (their weight for it is 0).
  * Results do not depend on the order in which the GPU runs the blocks.
+ * 16-bit rows: softmax statistics and sums are fp32; the weights are rounded to
+ * the rows' type before they meet the values (at most half a step of each), and
+ * kept with at least twice its bits where tcgen05 does not take the call: a page
+ * size that is no multiple of 8, a head dimension other than 64, 96, 128 and 256,
+ * more than 128 query heads per key head, expanded strides, a scaling not above 0.
+ * The waits inside the kernels give up after about a second: rows may then be
+ * wrong, and only KIV_ERRBIT_WAIT_TIMEOUT in `errors` tells.
  * fp32 rows are multiplied as sums of TF32 parts (22 bits of each product kept):
  * an infinite element of a row that some query sees gives NaN.
  */

@@ -104,7 +104,7 @@ class PagedQueryDesc(ctypes.Structure):
                 ("window", c_i32), ("scaling", c_f32), ("softcap", c_f32)]
 
 
-ERRBIT_BLOCK_TABLE, ERRBIT_SEQ_LEN, ERRBIT_POSITION = 32, 64, 128
+ERRBIT_WAIT_TIMEOUT, ERRBIT_BLOCK_TABLE, ERRBIT_SEQ_LEN, ERRBIT_POSITION = 8, 32, 64, 128
 
 P = ctypes.POINTER
 # name -> (restype, argtypes)

@@ -18,14 +18,16 @@
 // key tiles and one over the odd ones, and join at the end ("twins").  So the
 // same kernel serves decode, bound by memory: warps without rows only keep the
 // beat, and the tensor cores' empty rows cost nothing that is missed.  Measured
-// over 16 sequences of 16 k keys, one token each: 32/8 x 128 209 us (5.0 TB/s)
-// and 32/4 x 64 76 us, against 249 and 100 us for m16n8k16 products split over
-// the keys (paged_mma.cu); without twins 32/4 x 64 takes 97 us.
+// over 16 sequences of 16 k keys, one token each, pages of 128: 32/8 x 128 211 us
+// (5.1 TB/s) and 32/4 x 64 79 us, against 250 and 103 us for m16n8k16 products
+// split over the keys (paged_mma.cu); with pages of 16, 227 and 82 against 241
+// and 103; four times the sequences, 850 against 838.  Without twins 32/4 x 64
+// took 97 us where it took 76.
 // While one row tile's softmax runs, the tensor cores work on the other's
 // products, so both are kept busy: per tile pair the tensor cores need 4 x 512
 // cycles (D = 128) and the 2 x 16384 exponentials 2048 cycles of the special
-// function units.  Measured: 4096 tokens over 36864 keys, 32/8 x 128: 2.2-2.4 ms,
-// 0.92-1.06 PFLOP/s at the power limit (1.3-1.4 GHz); with the softmax taken out
+// function units.  Measured: 4096 tokens over 36864 keys, 32/8 x 128: 2.4-2.5 ms,
+// 0.93-0.97 PFLOP/s at the power limit (1.3-1.4 GHz); with the softmax taken out
 // the products alone take 1.6 ms.  One warp issuing both row tiles' products
 // took 3950 cycles per tile pair where this takes 3240.
 //

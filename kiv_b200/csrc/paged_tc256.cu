@@ -13,8 +13,9 @@
 // Per key tile the tensor cores need 1024 cycles for each product, the special
 // function units 1024 for the exponentials, and 128 KB come from L2: 62 bytes a
 // cycle, so the tensor cores and L2 share the bound.  Measured: two chunks of up
-// to 2047 tokens over up to 18 k keys, 8/1 x 256: 247-289 us, 1.0-1.18 PFLOP/s;
-// single tokens over pages of 16 read at 6.4 TB/s (one TMA warp: 4.0).
+// to 2047 tokens over up to 18 k keys, 8/1 x 256: 290 us, 1.0 PFLOP/s; single
+// tokens of 64 sequences of 32 k keys in pages of 16 read at 6.2 TB/s (one TMA
+// warp: 4.0).
 //
 // The rest (lazy rescale, dead rows, P over S in TMEM) is as in paged_tc.cu.
 #include <algorithm>

@@ -20,7 +20,10 @@ kernels read, so a call captured in a CUDA graph serves other lengths and pages
 on replay.  Rows behind ``q_starts[-1]`` (a padded batch) are neither read nor
 written.  ``errors`` (int64, optional) collects ``ERRBIT_*`` bits of
 ``kiv_b200._native``: page numbers, lengths and positions that the kernels
-could not follow -- they never read or write out of bounds.
+could not follow -- they never read or write out of bounds -- and
+``ERRBIT_WAIT_TIMEOUT``, a wait inside a kernel that gave up after about a
+second, which leaves rows of ``paged_attend`` wrong.  Without ``errors`` none of
+these is told (``PagedKVCache`` keeps one).
 
 Every call runs on the current stream of its tensors' device, allocates its
 scratch from that stream's pool and raises ``KIVNativeError`` on refused
@@ -138,7 +141,9 @@ def paged_attend(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
     the host knows it (chooses tilings, and so the order of fp32 sums, never which keys count or how exactly).  With
     ``return_lse`` also the float32 log-sum-exp of the scores ``[tokens, Hq]``; a row that sees no key gets 0 and -inf.
     Keys without a valid page read as rows of zeros.  Rows of ``out`` and ``lse`` behind ``q_starts[-1]`` are left as they
-    are.
+    are.  Statistics and sums are float32; with 16-bit rows the softmax weights are rounded to the rows' dtype before they
+    meet the values, and kept with at least twice its bits where the tcgen05 kernels do not take the call: a page size that
+    is no multiple of 8, a head dimension other than 64, 96, 128 and 256, more than 128 query heads per key head.
     """
     _refuse_gradients("paged_attend", q, k_pages, v_pages)
     if out is None:
